@@ -398,6 +398,115 @@ pkc_status pkc_relpos_attention_noalloc(const void* qkv, const void* ptab, int c
                                         int B, int d, int n_heads, int dtype, void* ctx,
                                         void* stream);
 
+/* ---- attention decoder (kernel-level entry points; device pointers)
+   What a decoder that attends to the encoder's output needs beside GEMMs:
+   cross attention, a key / value cache in 8 bits with the attention over it,
+   and beam search's selection and state reordering. No counterpart in the
+   reference (its decoders are CTC and transducers).
+
+   These calls are asynchronous: they launch on `stream` (a cudaStream_t, NULL
+   for the default stream), allocate nothing, keep nothing between calls and
+   can be captured into a graph; the arrays that they read (offsets, lengths,
+   tables) are read when the kernels run. `stream` must belong to the current
+   device, and so must the memory (PKC_ERR_ARG). A workspace belongs to one
+   call at a time: calls, or graphs, that may run at once need one each.
+
+   What only the device knows is checked there: an offset, length, page or
+   parent outside the sizes that the call was given leaves that item (for a
+   page: its tokens) out, and the first such error's code goes to *err, a
+   device int that the caller zeroes and reads when it likes (110: out of the
+   sizes, 111: a value that is not a number); err may be NULL. Rows that
+   belong to no item are left as they were.
+
+   Types: dtype 0 f16, 1 bf16 (beam_select also 2 f32); head_dim 64 or 128;
+   n_heads a multiple of n_kv_heads (query head h reads key head
+   h / (n_heads / n_kv_heads)). Row strides (ld*) are in elements. Rows start
+   on 16-byte boundaries: pointers 16-byte aligned, ld* multiples of 8. */
+
+/* Cross attention: item b's query rows [q_off[b], q_off[b+1]) of q attend to
+   the kv_len[b] rows of k and v from kv_off[b] on:
+   out = softmax(scale q k^T) v, f32 sums and softmax; an item without keys
+   gives zeros. q, out [q_rows][n_heads][head_dim]; k, v
+   [kv_rows][n_kv_heads][head_dim] (with row strides, so the k | v rows of one
+   projection need no copy); q_off [B + 1], kv_off, kv_len [B] int32 on the
+   device. max_q and max_kv bound the items' rows and keys. All of an item's
+   hypotheses are its query rows: they share one read of its keys. workspace:
+   pkc_cross_attention_workspace bytes, 16-byte aligned (NULL if 0). out may
+   not overlap the inputs. */
+pkc_status pkc_cross_attention(const void* q, long long ldq, const int* q_off, int max_q, int q_rows, const void* k,
+                               long long ldk, const void* v, long long ldv, const int* kv_off, const int* kv_len,
+                               int max_kv, int kv_rows, int B, int n_heads, int n_kv_heads, int head_dim, float scale,
+                               int dtype, void* out, long long ldo, void* workspace, size_t workspace_bytes, int* err,
+                               void* stream);
+size_t pkc_cross_attention_workspace(int B, int max_q, int max_kv, int n_heads, int n_kv_heads, int head_dim);
+
+/* A key / value cache in 8 bits, in pages. k and v hold e4m3 codes
+   [n_pages][n_kv_heads][page][head_dim]; k_scale and v_scale
+   [n_pages][n_kv_heads] f32 one power of two for each page and head: a value
+   is code * scale. table [n_seqs][table_ld] int32 gives the page of each
+   `page` tokens of a sequence. All on the device; page is 16, 32, 64 or 128.
+   Sequences may share full pages; a page that still fills belongs to one. The
+   struct itself is host memory, read during the call. */
+typedef struct pkc_kv8_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int* table;
+  int n_pages, page, n_kv_heads, head_dim, table_ld;
+} pkc_kv8_cache;
+
+/* Write new tokens: sequence s gets rows [new_off[s], new_off[s+1]) of k and v
+   ([rows][n_kv_heads][head_dim], 16-bit) as its last tokens; lens[s] counts
+   its tokens with them. max_new bounds a sequence's new tokens. A page's scale
+   is the smallest power of two (from 2^-126 on) under which its largest value
+   fits 448, and only grows: older codes of the page are rounded again under
+   the new scale (exact, but for codes that become subnormal). Values are
+   rounded to nearest even; an infinity takes the largest code, a NaN is stored
+   as 0 and reported (111). */
+pkc_status pkc_kv8_append(const pkc_kv8_cache* cache, const void* k, long long ldk, const void* v, long long ldv,
+                          const int* new_off, const int* lens, int n_seqs, int rows, int max_new, int dtype, int* err,
+                          void* stream);
+
+/* Causal self attention over the cache: the query rows [q_off[s], q_off[s+1])
+   are sequence s's last n tokens (appended before), so row i of n sees its
+   first lens[s] - n + i + 1 tokens. Other arguments as
+   pkc_cross_attention; max_len bounds lens. */
+pkc_status pkc_kv8_attention(const pkc_kv8_cache* cache, const void* q, long long ldq, const int* q_off, int max_q,
+                             int q_rows, const int* lens, int max_len, int n_seqs, int n_heads, float scale, int dtype,
+                             void* out, long long ldo, void* workspace, size_t workspace_bytes, int* err, void* stream);
+size_t pkc_kv8_attention_workspace(const pkc_kv8_cache* cache, int n_seqs, int max_q, int max_len, int n_heads);
+
+/* The cache follows a beam search's hypotheses, in place: sequence b*K + k
+   becomes a copy of what sequence b*K + parent[b*K + k] was. Full pages are
+   shared (table entries), the page that still fills is copied into the
+   sequence's own. lens[B*K]: the K sequences of an item have one length and K
+   different pages to fill. K <= 32. */
+pkc_status pkc_kv8_reorder(const pkc_kv8_cache* cache, const int* parent, const int* lens, int B, int K, int* err,
+                           void* stream);
+
+/* One selection step of beam search over B items of K hypotheses (K <= 32):
+   the K best of cum[b, j] + log_softmax(logits[b*K + j])[v] over all j and v
+   (ties: the lowest j*V + v), best first. cum, score [B, K] f32 (sums and
+   scores are formed in f64 and rounded once), finished [B, K] uint8 or NULL: a
+   finished hypothesis offers itself alone, with token eos and its score.
+   parent, token [B, K] int32; finished_out [B, K] (or NULL): token is eos, or
+   the parent had finished. A row with a NaN or +inf, or all -inf, and a NaN in
+   cum offer -inf. score may be cum, finished_out may be finished; logits row
+   stride ld. At the first step give hypotheses 1 .. K-1 a cum of -inf. */
+pkc_status pkc_beam_select(const void* logits, long long ld, int dtype, const float* cum, const uint8_t* finished,
+                           int B, int K, int V, int eos, float* score, int* parent, int* token, uint8_t* finished_out,
+                           void* stream);
+
+/* States follow their hypotheses, in place: row b*K + k of each of n_outer
+   blocks becomes a copy of what row b*K + parent[b*K + k] was. Rows are
+   row_bytes long, row_stride bytes apart, blocks outer_stride bytes (any
+   alignment; 16 is fastest). lens (or NULL): only the first
+   lens[b] * unit_bytes of a row are live. K <= 32. */
+pkc_status pkc_beam_reorder(void* state, const int* parent, int B, int K, long long row_bytes, long long row_stride,
+                            int n_outer, long long outer_stride, const int* lens, long long unit_bytes, int* err,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -67,6 +67,13 @@ class KernelStat(ctypes.Structure):
                 ("flops", c_double), ("bytes", c_double)]
 
 
+class KV8Cache(ctypes.Structure):
+    """pkc_kv8_cache: a paged key / value cache in 8 bits (device pointers as
+    ints). The caller owns the memory."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("table", c_void_p),
+                ("n_pages", c_int), ("page", c_int), ("n_kv_heads", c_int), ("head_dim", c_int), ("table_ld", c_int)]
+
+
 _lib = None
 
 
@@ -143,6 +150,20 @@ def _declare(L):
         ("pkc_bounded_wait_check", c_int, c_int, ctypes.c_double, POINTER(c_int)),
         ("pkc_conv_depthwise", c_int, c_void_p, POINTER(c_int), c_int, c_int, c_int, c_void_p, c_void_p,
          c_void_p, c_void_p, c_int, c_void_p, c_void_p),
+        ("pkc_cross_attention", c_int, c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p,
+         c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p,
+         c_longlong, c_void_p, c_size_t, c_void_p, c_void_p),
+        ("pkc_cross_attention_workspace", c_size_t, c_int, c_int, c_int, c_int, c_int, c_int),
+        ("pkc_kv8_append", c_int, POINTER(KV8Cache), c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p,
+         c_int, c_int, c_int, c_int, c_void_p, c_void_p),
+        ("pkc_kv8_attention", c_int, POINTER(KV8Cache), c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p,
+         c_int, c_int, c_int, c_float, c_int, c_void_p, c_longlong, c_void_p, c_size_t, c_void_p, c_void_p),
+        ("pkc_kv8_attention_workspace", c_size_t, POINTER(KV8Cache), c_int, c_int, c_int, c_int),
+        ("pkc_kv8_reorder", c_int, POINTER(KV8Cache), c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p),
+        ("pkc_beam_select", c_int, c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p),
+        ("pkc_beam_reorder", c_int, c_void_p, c_void_p, c_int, c_int, c_longlong, c_longlong, c_int, c_longlong,
+         c_void_p, c_longlong, c_void_p, c_void_p),
     ]
     for name, res, *args in optional:
         if hasattr(L, name):
@@ -251,6 +272,78 @@ def relpos_attention_noalloc(qkv, ptab, centre, bias_u, bias_v, lens, d, n_heads
                                               c_void_p(bias_v), _ints(lens), len(lens), d, n_heads,
                                               1 if bf16 else 0, c_void_p(ctx),
                                               c_void_p(stream) if stream else None))
+
+
+# ---- attention decoder: asynchronous on `stream`, device pointers as ints (0: NULL)
+
+DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
+_DTYPES = {"f16": DTYPE_F16, "bf16": DTYPE_BF16, "f32": DTYPE_F32}
+
+
+def _scale(head_dim, scale):
+    if scale is not None:
+        return scale
+    return head_dim ** -0.5 if head_dim > 0 else 0.0
+
+
+def cross_attention_workspace(B, max_q, max_kv, n_heads, n_kv_heads, head_dim):
+    """Workspace bytes of cross_attention for calls of these sizes."""
+    return int(lib().pkc_cross_attention_workspace(B, max_q, max_kv, n_heads, n_kv_heads, head_dim))
+
+
+def cross_attention(q, k, v, q_off, kv_off, kv_len, B, n_heads, n_kv_heads, head_dim, *, q_rows, kv_rows, max_q,
+                    max_kv, bf16, out, ldq=None, ldk=None, ldv=None, ldo=None, scale=None, workspace=0,
+                    workspace_bytes=0, err=0, stream=0):
+    """Attention of packed query rows to the encoder's states of their item
+    (scale defaults to head_dim ** -0.5)."""
+    _check(lib().pkc_cross_attention(
+        q, n_heads * head_dim if ldq is None else ldq, q_off, max_q, q_rows,
+        k, n_kv_heads * head_dim if ldk is None else ldk, v, n_kv_heads * head_dim if ldv is None else ldv,
+        kv_off, kv_len, max_kv, kv_rows, B, n_heads, n_kv_heads, head_dim,
+        _scale(head_dim, scale), 1 if bf16 else 0,
+        out, n_heads * head_dim if ldo is None else ldo, workspace, workspace_bytes, err, stream))
+
+
+def kv8_append(cache, k, v, new_off, lens, n_seqs, *, rows, max_new, bf16, ldk=None, ldv=None, err=0, stream=0):
+    """Write new tokens' keys and values into a KV8Cache."""
+    ld = cache.n_kv_heads * cache.head_dim
+    _check(lib().pkc_kv8_append(cache, k, ld if ldk is None else ldk, v, ld if ldv is None else ldv, new_off, lens,
+                                n_seqs, rows, max_new, 1 if bf16 else 0, err, stream))
+
+
+def kv8_attention_workspace(cache, n_seqs, max_q, max_len, n_heads):
+    """Workspace bytes of kv8_attention for calls of these sizes."""
+    return int(lib().pkc_kv8_attention_workspace(cache, n_seqs, max_q, max_len, n_heads))
+
+
+def kv8_attention(cache, q, q_off, lens, n_seqs, n_heads, *, q_rows, max_q, max_len, bf16, out, ldq=None, ldo=None,
+                  scale=None, workspace=0, workspace_bytes=0, err=0, stream=0):
+    """Causal attention of each sequence's last tokens over its cache."""
+    D = cache.head_dim
+    _check(lib().pkc_kv8_attention(cache, q, n_heads * D if ldq is None else ldq, q_off, max_q, q_rows, lens, max_len,
+                                   n_seqs, n_heads, _scale(D, scale), 1 if bf16 else 0, out,
+                                   n_heads * D if ldo is None else ldo, workspace, workspace_bytes, err, stream))
+
+
+def kv8_reorder(cache, parent, lens, B, K, *, err=0, stream=0):
+    """The cache follows a beam search's hypotheses, in place."""
+    _check(lib().pkc_kv8_reorder(cache, parent, lens, B, K, err, stream))
+
+
+def beam_select(logits, cum, finished, B, K, V, *, eos, score, parent, token, dtype="f32", finished_out=0, ld=None,
+                stream=0):
+    """One selection step of beam search (dtype of the logits: "f16", "bf16" or "f32")."""
+    _check(lib().pkc_beam_select(logits, V if ld is None else ld, _DTYPES[dtype], cum, finished, B, K, V, eos, score,
+                                 parent, token, finished_out, stream))
+
+
+def beam_reorder(state, parent, B, K, *, row_bytes, row_stride=None, n_outer=1, outer_stride=None, lens=0,
+                 unit_bytes=0, err=0, stream=0):
+    """State rows follow a beam search's hypotheses, in place."""
+    row_stride = row_bytes if row_stride is None else row_stride
+    _check(lib().pkc_beam_reorder(state, parent, B, K, row_bytes, row_stride, n_outer,
+                                  B * K * row_stride if outer_stride is None else outer_stride, lens, unit_bytes, err,
+                                  stream))
 
 
 def pack_cache_build(gguf_path: str, cache_dir: str) -> str:
