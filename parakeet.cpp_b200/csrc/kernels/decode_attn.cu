@@ -6,17 +6,19 @@
 //
 // Such a call reads every key and value once for at most a few rows, so it is
 // bound by memory: one CTA takes up to 16 rows (tokens x heads of one shared
-// key head) of one item and one part of its keys; its four warps walk tiles of
-// WT keys on their own, each with its own running maximum and sum. Parts are
-// joined by k_attn_join when there is more than one.
+// key head) of one item and one part of its keys; its warps walk tiles of WT
+// keys on their own, each with its own ring of tiles in shared memory (filled
+// by cp.async two tiles ahead, no barrier but the warp's own) and its own
+// running maximum and sum. Parts are joined by k_attn_join when there is more
+// than one.
 //
-// Fragments come from global memory straight into registers, 16 bytes a load:
-// the order of the contraction is free as long as both operands share it, so a
-// thread of mma.m16n8k16 that owns key n = lane / 4 takes 16 contiguous bytes
-// of that key's row and the query fragments are loaded in the same order; for
-// P V it takes 16 contiguous bytes of each of its four keys' value rows, whose
-// elements belong to different 8-column tiles of the product. No shared memory
-// and no transposition lies between the load and the product.
+// Fragments are 16-byte reads of the tile as it lies in memory: the order of
+// the contraction is free as long as both operands share it, so a thread of
+// mma.m16n8k16 that owns key n = lane / 4 takes 16 contiguous bytes of that
+// key's row and the query fragments are loaded in the same order; for P V it
+// takes 16 contiguous bytes of each of its four keys' value rows, whose
+// elements belong to different 8-column tiles of the product. No transposition
+// lies between the copy and the product.
 //
 // 8-bit codes become f16 exactly (cvt e4m3x2 -> f16x2). A tile lies in one
 // page, so its two scales are scalars: the key scale goes into the softmax's
@@ -32,8 +34,8 @@ namespace pkc {
 
 namespace {
 
-constexpr int kWarps = 4;
 constexpr int kRows = 16;
+constexpr int kStages = 3;  // tiles in a warp's ring
 constexpr int kSms = 148;
 
 template <typename M>
@@ -93,15 +95,51 @@ __device__ __forceinline__ long long part_at(const DecodeAttnArgs& a, int row_ti
   return ((long long)b * a.n_kv_heads + h) * row_tiles + rt;
 }
 
-// H: type of q and out; Q8: 8-bit cache, else keys and values of type H.
-template <typename H, bool Q8, int D, int WT>
-__global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const DecodeAttnArgs a, int row_tiles, int n_split) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Where 16-byte chunk ch of row r of a tile lies. The reads below take, at a
+// time, four chunks of two neighbouring rows (keys) or two chunks of rows 0, 2,
+// 4, 6 of eight (values): these permutations give each such set eight
+// different chunk columns of 128 bytes.
+template <int RB>
+__device__ __forceinline__ int key_at(int r, int ch) {
+  return RB == 64 ? r * 64 + ch * 16 : r * RB + (ch ^ ((r & 1) << 2)) * 16;
+}
+template <int RB>
+__device__ __forceinline__ int value_at(int r, int ch) {
+  return RB == 64 ? (r ^ ((r >> 2) & 1)) * 64 + (ch ^ (r & 2)) * 16 : r * RB + (ch ^ (r & 6)) * 16;
+}
+
+// Shared memory of a CTA of W warps: the rings, then each stage's two scales;
+// the join of the warps reuses the rings.
+template <int RB, int WT>
+struct RowsLayout {
+  static constexpr int kTile = WT * RB;  // keys or values of a tile
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kWarp = kStages * kStage + kStages * 16;  // + {key scale, value scale}
+};
+
+// H: type of q and out; Q8: 8-bit cache, else keys and values of type H; W
+// warps share the CTA's part of the keys.
+template <typename H, bool Q8, int D, int WT, int W>
+__global__ void __launch_bounds__(32 * W, 8 / W) k_attn_rows(const DecodeAttnArgs a, int row_tiles, int n_split) {
   using M = typename std::conditional<Q8, __half, H>::type;  // type of the products
-  constexpr int KC = Q8 ? D / 64 : D / 32;                   // 16-byte loads of a key row, per thread
-  constexpr int VW = Q8 ? D / 32 : D / 16;                   // 32-bit words of a value row, per thread
+  constexpr int RB = Q8 ? D : 2 * D;                         // bytes of a row
+  constexpr int KC = RB / 64;                                // 16-byte reads of a key row, per thread
+  constexpr int VW = RB / 32;                                // 32-bit words of a value row, per thread
   constexpr int NT = D / 8;                                  // 8-column tiles of the output
-  __shared__ float s_o[kWarps][kRows][D + 4];
-  __shared__ float s_ml[kWarps][kRows][2];
+  using L = RowsLayout<RB, WT>;
+  extern __shared__ __align__(128) uint8_t smem[];
 
   const int G = a.n_heads / a.n_kv_heads;
   const int split = blockIdx.x % n_split;
@@ -109,7 +147,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const DecodeAttnArgs 
   const int rt = rest % row_tiles;
   rest /= row_tiles;
   const int h = rest % a.n_kv_heads, b = rest / a.n_kv_heads;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int warp = W == 1 ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   pdl_wait();
   pdl_trigger();
   const Item it = load_item<Q8>(a, b);
@@ -119,6 +157,81 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const DecodeAttnArgs 
   }
   const int rows = it.n * G;
   if (rt * kRows >= rows) return;
+
+  // ---- this warp's tiles: t_begin + warp, + W, ...
+  // the last row's last key ends the walk
+  const int last = min(rows, (rt + 1) * kRows) - 1;
+  const int vmax = max(0, visible<Q8>(it, last / G));
+  const int n_tiles = (vmax + WT - 1) / WT;
+  const int per = (n_tiles + n_split - 1) / n_split;
+  const int t0 = split * per + warp, t_end = min(n_tiles, (split + 1) * per);
+  const int cnt = t0 < t_end ? (t_end - t0 + W - 1) / W : 0;
+  uint8_t* ring = smem + warp * L::kWarp;
+  const uint32_t ring_s = smem_u32(ring);
+  const uint8_t* kbase = nullptr;
+  const uint8_t* vbase = nullptr;
+  if constexpr (!Q8) {
+    kbase = reinterpret_cast<const uint8_t*>(reinterpret_cast<const H*>(a.k) + (long long)it.kv0 * a.ldk + h * D);
+    vbase = reinterpret_cast<const uint8_t*>(reinterpret_cast<const H*>(a.v) + (long long)it.kv0 * a.ldv + h * D);
+  }
+  auto page_of = [&](int i) -> int {  // page of the warp's i-th tile
+    if constexpr (!Q8) return 0;
+    if (i >= cnt) return 0;
+    return a.cache.table[(long long)b * a.cache.table_ld + (t0 + W * i) * WT / a.cache.page];
+  };
+  // copy the warp's i-th tile; rows that no query row sees become zeros (a NaN
+  // there would survive a probability of zero)
+  auto issue = [&](int i, int id) {
+    if (i < cnt) {
+      const int k0 = (t0 + W * i) * WT, left = vmax - k0;
+      const uint32_t dst = ring_s + (i % kStages) * L::kStage;
+      const uint8_t *kp = kbase, *vp = vbase;
+      long long kst = RB, vst = RB;
+      bool on = true;
+      if constexpr (Q8) {
+        const Kv8& cc = a.cache;
+        on = id >= 0 && id < cc.n_pages;
+        const long long ph = (long long)(on ? id : 0) * cc.n_kv_heads + h;
+        kp = cc.k + (ph * cc.page + k0 % cc.page) * D;
+        vp = cc.v + (ph * cc.page + k0 % cc.page) * D;
+        const uint32_t sc = ring_s + kStages * L::kStage + (i % kStages) * 16;
+        if (on) {
+          if (lane < 2) cp_async4(sc + 4 * lane, (lane ? cc.v_scale : cc.k_scale) + ph);
+        } else if (lane == 0) {
+          // the keys of a page that is none are not seen
+          report_error(a.err, DEV_ERR_BAD_SHAPE);
+          *reinterpret_cast<float*>(ring + kStages * L::kStage + (i % kStages) * 16) = -1.f;
+        }
+      } else {
+        kst = a.ldk * 2;
+        vst = a.ldv * 2;
+        kp += k0 * kst;
+        vp += k0 * vst;
+      }
+#pragma unroll
+      for (int j = 0; j < L::kTile / 512; ++j) {
+        const int q = j * 32 + lane, r = q / (RB / 16), ch = q % (RB / 16);
+        const bool in = on && r < left;
+        cp_async16(dst + key_at<RB>(r, ch), kp + (in ? r : 0) * kst + ch * 16, in ? 16 : 0);
+      }
+#pragma unroll
+      for (int j = 0; j < L::kTile / 512; ++j) {
+        const int q = j * 32 + lane, r = q / (RB / 16), ch = q % (RB / 16);
+        const bool in = on && r < left;
+        cp_async16(dst + L::kTile + value_at<RB>(r, ch), vp + (in ? r : 0) * vst + ch * 16, in ? 16 : 0);
+      }
+    }
+    cp_commit();
+  };
+  int id_next;
+  {
+    int ids[kStages];
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) ids[i] = page_of(i);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i, ids[i]);
+    id_next = ids[kStages - 1];
+  }
 
   // ---- queries: rows g and g + 8 of the tile, in the key loads' order
   uint32_t qf[D / 16][4];
@@ -170,13 +283,6 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const DecodeAttnArgs 
       qf[2 * j + 1][2 + e] = w[j].w;
     }
   }
-  // the last row's last key ends the walk
-  const int last = min(rows, (rt + 1) * kRows) - 1;
-  const int vmax = max(0, visible<Q8>(it, last / G));
-  const int n_tiles = (vmax + WT - 1) / WT;
-  const int per = (n_tiles + n_split - 1) / n_split;
-  const int t_end = min(n_tiles, (split + 1) * per);
-
   float o[NT][4];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -184,62 +290,20 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const DecodeAttnArgs 
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-  for (int t = split * per + warp; t < t_end; t += kWarps) {
-    const int k0 = t * WT;
-    // ---- this tile's rows
-    const uint8_t *kp, *vp;
-    long long kst, vst;  // bytes between keys
+  for (int i = 0; i < cnt; ++i) {
+    cp_wait<kStages - 2>();
+    __syncwarp();
+    issue(i + kStages - 1, id_next);
+    id_next = page_of(i + kStages);
+    const int k0 = (t0 + W * i) * WT;
+    const uint8_t* kt = ring + (i % kStages) * L::kStage;
+    const uint8_t* vt = kt + L::kTile;
     float ks = 1.f, vs = 1.f;
     if constexpr (Q8) {
-      const Kv8& cc = a.cache;
-      const int pg = k0 / cc.page;
-      const int id = cc.table[(long long)b * cc.table_ld + pg];
-      if (id < 0 || id >= cc.n_pages) {
-        if (lane == 0) report_error(a.err, DEV_ERR_BAD_SHAPE);
-        continue;  // the keys of a page that is none are not seen
-      }
-      const long long ph = (long long)id * cc.n_kv_heads + h;
-      kp = cc.k + (ph * cc.page + (k0 - pg * cc.page)) * D;
-      vp = cc.v + (ph * cc.page + (k0 - pg * cc.page)) * D;
-      kst = vst = D;
-      ks = cc.k_scale[ph];
-      vs = cc.v_scale[ph];
-    } else {
-      kp = reinterpret_cast<const uint8_t*>(reinterpret_cast<const H*>(a.k) + (long long)(it.kv0 + k0) * a.ldk + h * D);
-      vp = reinterpret_cast<const uint8_t*>(reinterpret_cast<const H*>(a.v) + (long long)(it.kv0 + k0) * a.ldv + h * D);
-      kst = a.ldk * 2;
-      vst = a.ldv * 2;
-    }
-    const int left = vmax - k0;  // keys of this tile that any row sees (>= 1)
-    uint4 kr[WT / 8][KC];
-#pragma unroll
-    for (int i = 0; i < WT / 8; ++i) {
-      const int key = min(8 * i + g, left - 1);
-#pragma unroll
-      for (int j = 0; j < KC; ++j) kr[i][j] = *reinterpret_cast<const uint4*>(kp + key * kst + j * 64 + c * 16);
-    }
-    // values: keys 16 i + {0, 1, 8, 9} + 2 c; what no row sees is zero, not
-    // whatever lies there (zero times a NaN would be one)
-    uint32_t vr[WT / 4][VW];
-#pragma unroll
-    for (int i = 0; i < WT / 4; ++i) {
-      const int key = 16 * (i >> 2) + 2 * c + (i & 1) + 8 * ((i >> 1) & 1);
-      const bool on = key < left;
-      const uint8_t* p = vp + (on ? key : 0) * vst;
-      if constexpr (VW == 2) {
-        const uint2 x = *reinterpret_cast<const uint2*>(p + g * 8);
-        vr[i][0] = on ? x.x : 0u;
-        vr[i][1] = on ? x.y : 0u;
-      } else {
-#pragma unroll
-        for (int j = 0; j < VW / 4; ++j) {
-          const uint4 x = *reinterpret_cast<const uint4*>(p + j * 128 + g * 16);
-          vr[i][4 * j] = on ? x.x : 0u;
-          vr[i][4 * j + 1] = on ? x.y : 0u;
-          vr[i][4 * j + 2] = on ? x.z : 0u;
-          vr[i][4 * j + 3] = on ? x.w : 0u;
-        }
-      }
+      const float* sc = reinterpret_cast<const float*>(ring + kStages * L::kStage + (i % kStages) * 16);
+      ks = sc[0];
+      vs = sc[1];
+      if (ks < 0.f) continue;
     }
     // ---- scores
     float s[WT / 8][4];
@@ -248,7 +312,8 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const DecodeAttnArgs 
       s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
-        const uint32_t w[4] = {kr[i][j].x, kr[i][j].y, kr[i][j].z, kr[i][j].w};
+        const uint4 kr = *reinterpret_cast<const uint4*>(kt + key_at<RB>(8 * i + g, 4 * j + c));
+        const uint32_t w[4] = {kr.x, kr.y, kr.z, kr.w};
         if constexpr (Q8) {
 #pragma unroll
           for (int u = 0; u < 4; ++u) mma16816<M>(s[i], qf[4 * j + u], e4m3_lo(w[u]), e4m3_hi(w[u]));
@@ -297,7 +362,26 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const DecodeAttnArgs 
       pf[i >> 1][2 * (i & 1)] = pack2<M>(s[i][0], s[i][1]);
       pf[i >> 1][2 * (i & 1) + 1] = pack2<M>(s[i][2], s[i][3]);
     }
-    // ---- values
+    // ---- values: keys 16 i + {0, 1, 8, 9} + 2 c
+    uint32_t vr[WT / 4][VW];
+#pragma unroll
+    for (int i = 0; i < WT / 4; ++i) {
+      const int r = 16 * (i >> 2) + 2 * c + (i & 1) + 8 * ((i >> 1) & 1);
+      if constexpr (VW == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(vt + value_at<RB>(r, g >> 1) + (g & 1) * 8);
+        vr[i][0] = x.x;
+        vr[i][1] = x.y;
+      } else {
+#pragma unroll
+        for (int j = 0; j < VW / 4; ++j) {
+          const uint4 x = *reinterpret_cast<const uint4*>(vt + value_at<RB>(r, 8 * j + g));
+          vr[i][4 * j] = x.x;
+          vr[i][4 * j + 1] = x.y;
+          vr[i][4 * j + 2] = x.z;
+          vr[i][4 * j + 3] = x.w;
+        }
+      }
+    }
     if constexpr (Q8) {
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
@@ -331,52 +415,88 @@ __global__ void __launch_bounds__(32 * kWarps) k_attn_rows(const DecodeAttnArgs 
     }
   }
 
-  // ---- join the warps
+  // ---- what this warp holds of rows g (e = 0) and g + 8: four columns at a time
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
     l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-    if (c == 0) {
-      s_ml[warp][g + 8 * e][0] = m[e];
-      s_ml[warp][g + 8 * e][1] = l[e];
-    }
   }
+  auto each = [&](auto&& f) {
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int n = 2 * c + (e & 1);  // column n of tile i
-      const int dim = Q8 ? n * (D / 8) + i : (i >> 3) * 64 + n * 8 + (i & 7);
-      s_o[warp][g + 8 * (e >> 1)][dim] = o[i][e];
-    }
-  __syncthreads();
+      for (int n = 0; n < 2; ++n)  // column 2 c + n of the 8-column tiles
+#pragma unroll
+        for (int i = 0; i < NT; i += 4) {
+          const int dim = Q8 ? (2 * c + n) * (D / 8) + i : (i >> 3) * 64 + (2 * c + n) * 8 + (i & 7);
+          const int x = 2 * e + n;
+          f(e, dim, make_float4(o[i][x], o[i + 1][x], o[i + 2][x], o[i + 3][x]));
+        }
+  };
   const int valid = min(kRows, rows - rt * kRows);
-  const long long part = part_at(a, row_tiles, b, h, rt) * n_split + split;
-  float* po = a.ws + part * (kRows * (D + 2));
-  for (int idx = threadIdx.x; idx < valid * (D / 4); idx += 32 * kWarps) {
-    const int r = idx / (D / 4), d4 = idx % (D / 4) * 4;
-    float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_ml[w][r][0]);
-    const float base = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2_approx(s_ml[w][r][0] - base);
-      ll += s_ml[w][r][1] * f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = fmaf(s_o[w][r][d4 + e], f, x[e]);
-    }
+  float* po = a.ws + (part_at(a, row_tiles, b, h, rt) * n_split + split) * (kRows * (D + 2));
+  auto store_out = [&](int r, int dim, float4 v) {
+    const int row = rt * kRows + r;
+    H* op = reinterpret_cast<H*>(a.out) + (long long)(it.q0 + row / G) * a.ldo + (h * G + row % G) * D + dim;
+    *reinterpret_cast<uint2*>(op) = make_uint2(pack2<H>(v.x, v.y), pack2<H>(v.z, v.w));
+  };
+  if constexpr (W == 1) {
     if (n_split == 1) {
-      const int row = rt * kRows + r;
-      H* op = reinterpret_cast<H*>(a.out) + (long long)(it.q0 + row / G) * a.ldo + (h * G + row % G) * D + d4;
-      const float inv = ll == 0.f ? 0.f : 1.f / ll;  // no key seen: zeros
-      *reinterpret_cast<uint2*>(op) = make_uint2(pack2<H>(x[0] * inv, x[1] * inv), pack2<H>(x[2] * inv, x[3] * inv));
+      float inv[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) inv[e] = l[e] == 0.f ? 0.f : 1.f / l[e];  // no key seen: zeros
+      each([&](int e, int dim, float4 v) {
+        if (g + 8 * e < valid)
+          store_out(g + 8 * e, dim, make_float4(v.x * inv[e], v.y * inv[e], v.z * inv[e], v.w * inv[e]));
+      });
     } else {
-      *reinterpret_cast<float4*>(po + r * D + d4) = make_float4(x[0], x[1], x[2], x[3]);
-      if (d4 == 0) {
-        po[kRows * D + 2 * r] = mm;
-        po[kRows * D + 2 * r + 1] = ll;
+      each([&](int e, int dim, float4 v) {
+        if (g + 8 * e < valid) *reinterpret_cast<float4*>(po + (g + 8 * e) * D + dim) = v;
+      });
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (c == 0 && g + 8 * e < valid)
+          *reinterpret_cast<float2*>(po + kRows * D + 2 * (g + 8 * e)) = make_float2(m[e], l[e]);
+    }
+  } else {
+    // ---- join the warps, in the rings' memory
+    cp_wait<0>();
+    __syncthreads();
+    constexpr int LD = D + 4;
+    float* s_o = reinterpret_cast<float*>(smem);          // [W][kRows][LD]
+    float* s_ml = s_o + W * kRows * LD;                   // [W][kRows][2]
+    static_assert((W * kRows * (LD + 2)) * 4 <= W * L::kWarp, "the join fits the rings");
+    each([&](int e, int dim, float4 v) {
+      *reinterpret_cast<float4*>(s_o + (warp * kRows + g + 8 * e) * LD + dim) = v;
+    });
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (c == 0)
+        *reinterpret_cast<float2*>(s_ml + (warp * kRows + g + 8 * e) * 2) = make_float2(m[e], l[e]);
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < valid * (D / 4); idx += 32 * W) {
+      const int r = idx / (D / 4), d4 = idx % (D / 4) * 4;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < W; ++w) mm = fmaxf(mm, s_ml[(w * kRows + r) * 2]);
+      const float base = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float f = ex2_approx(s_ml[(w * kRows + r) * 2] - base);
+        ll += s_ml[(w * kRows + r) * 2 + 1] * f;
+        const float4 v = *reinterpret_cast<const float4*>(s_o + (w * kRows + r) * LD + d4);
+        x[0] = fmaf(v.x, f, x[0]);
+        x[1] = fmaf(v.y, f, x[1]);
+        x[2] = fmaf(v.z, f, x[2]);
+        x[3] = fmaf(v.w, f, x[3]);
+      }
+      if (n_split == 1) {
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        store_out(r, d4, make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv));
+      } else {
+        *reinterpret_cast<float4*>(po + r * D + d4) = make_float4(x[0], x[1], x[2], x[3]);
+        if (d4 == 0) *reinterpret_cast<float2*>(po + kRows * D + 2 * r) = make_float2(mm, ll);
       }
     }
   }
@@ -415,13 +535,20 @@ __global__ void __launch_bounds__(kRows * D / 4) k_attn_join(const DecodeAttnArg
   *reinterpret_cast<uint2*>(op) = make_uint2(pack2<H>(x[0] * inv, x[1] * inv), pack2<H>(x[2] * inv, x[3] * inv));
 }
 
-// Parts of each item's keys: enough CTAs for about four on every SM, and at
-// least 128 keys in a part.
-int plan_splits(long long blocks, int max_kv) {
-  const long long want = (4LL * kSms + blocks - 1) / blocks;
+// How a call is cut: `warps` a CTA and parts of each item's keys.
+//  - Many blocks of rows: a warp takes one alone (CTAs of one warp, no join).
+//  - Else four warps share a part, and the keys are cut into as many parts as
+//    give about six CTAs an SM (lengths differ; two run at a time), of at
+//    least 128 keys.
+struct Plan {
+  int warps, n_split;
+};
+Plan plan_rows(long long blocks, int max_kv) {
+  if (blocks >= 8LL * kSms) return {1, 1};
+  const long long want = (6LL * kSms + blocks - 1) / blocks;
   const long long most = (max_kv + 127) / 128;
   const long long n = want < most ? want : most;
-  return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+  return {4, n < 1 ? 1 : n > 64 ? 64 : (int)n};
 }
 
 long long row_blocks(int n_items, int max_q, int n_heads, int n_kv_heads, int* row_tiles) {
@@ -429,16 +556,29 @@ long long row_blocks(int n_items, int max_q, int n_heads, int n_kv_heads, int* r
   return (long long)n_items * n_kv_heads * *row_tiles;
 }
 
+template <typename H, bool Q8, int D, int WT, int W>
+cudaError_t launch_w(const DecodeAttnArgs& a, long long blocks, int rt, int n_split, cudaStream_t st) {
+  auto kern = k_attn_rows<H, Q8, D, WT, W>;
+  constexpr int smem = W * RowsLayout<Q8 ? D : 2 * D, WT>::kWarp;
+  static PerDevice once;
+  int unused = 0;
+  const cudaError_t e = per_device(once, &unused, [&](int, int&) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  });
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kern, dim3((unsigned)(blocks * n_split)), dim3(32 * W), smem, st, a, rt, n_split);
+}
+
 template <typename H, bool Q8, int D, int WT>
 cudaError_t launch_rows(const DecodeAttnArgs& a, cudaStream_t st) {
   int rt = 0;
   const long long blocks = row_blocks(a.n_items, a.max_q, a.n_heads, a.n_kv_heads, &rt);
-  const int n_split = plan_splits(blocks, a.max_kv);
-  if (blocks * n_split > 0x7fffffffLL) return cudaErrorInvalidValue;
-  cudaError_t e = launch_pdl(k_attn_rows<H, Q8, D, WT>, dim3((unsigned)(blocks * n_split)), dim3(32 * kWarps), 0, st, a,
-                             rt, n_split);
-  if (e != cudaSuccess || n_split == 1) return e;
-  return launch_pdl(k_attn_join<H, Q8, D>, dim3((unsigned)blocks), dim3(kRows * D / 4), 0, st, a, rt, n_split);
+  const Plan p = plan_rows(blocks, a.max_kv);
+  if (blocks * p.n_split > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const cudaError_t e = p.warps == 1 ? launch_w<H, Q8, D, WT, 1>(a, blocks, rt, p.n_split, st)
+                                     : launch_w<H, Q8, D, WT, 4>(a, blocks, rt, p.n_split, st);
+  if (e != cudaSuccess || p.n_split == 1) return e;
+  return launch_pdl(k_attn_join<H, Q8, D>, dim3((unsigned)blocks), dim3(kRows * D / 4), 0, st, a, rt, p.n_split);
 }
 
 template <typename H>
@@ -457,7 +597,7 @@ size_t decode_attn_ws_bytes(int n_items, int max_q, int max_kv, int n_heads, int
   int rt = 0;
   const long long blocks = row_blocks(n_items, max_q, n_heads, n_kv_heads, &rt);
   if (blocks <= 0) return 0;
-  const int n_split = plan_splits(blocks, max_kv);
+  const int n_split = plan_rows(blocks, max_kv).n_split;
   return n_split == 1 ? 0 : (size_t)blocks * n_split * kRows * (head_dim + 2) * sizeof(float);
 }
 
