@@ -12,20 +12,30 @@
 // running maximum and sum. Parts are joined by k_attn_join when there is more
 // than one.
 //
+// The products are taken transposed, S^T = K Q^T and O^T = V^T P^T: keys and
+// then output columns fill the 16 rows of mma.m16n8k16 and the few query rows
+// its 8 columns, so eight rows cost half of what 16 do (rows as the 16-row
+// side: 850 instructions a tile of 32 keys instead of about 400, and twice the
+// accumulators). P^T goes from the accumulator's layout to the operand's by
+// movmatrix.
+//
 // Fragments are 16-byte reads of the tile as it lies in memory: the order of
-// the contraction is free as long as both operands share it, so a thread of
-// mma.m16n8k16 that owns key n = lane / 4 takes 16 contiguous bytes of that
-// key's row and the query fragments are loaded in the same order; for P V it
-// takes 16 contiguous bytes of each of its four keys' value rows, whose
-// elements belong to different 8-column tiles of the product. No transposition
-// lies between the copy and the product.
+// the contraction is free as long as both operands share it, so a thread that
+// owns key lane / 4 takes 16 contiguous bytes of that key's row and the query
+// fragments are loaded in the same order; for V^T it takes 16 contiguous bytes
+// of each of its four keys' value rows, whose elements belong to different
+// rows of the product's tiles. No transposition lies between the copy and the
+// product.
 //
 // 8-bit codes become f16 exactly (cvt e4m3x2 -> f16x2). A tile lies in one
-// page, so its two scales are scalars: the key scale goes into the softmax's
-// factor, the value scale (a power of two) multiplies the tile's product in
-// f32, where it cannot under- or overflow as it could in f16 probabilities.
-// bf16 queries are brought to f16 with a power of two for each row (their 8
-// bits fit f16's 11), which the softmax's factor takes back.
+// page, so its two scales are scalars. The key scale goes into the softmax's
+// factor. The value scale, a power of two, goes into the exponent of the
+// probabilities as the difference to a reference exponent in which the output
+// is kept, as long as the page is at most 2^4 below it (the reference rises
+// with the pages); values of a page further below would lose bits of their f16
+// probabilities and take a product of their own, scaled in f32. bf16 queries
+// are brought to f16 with a power of two for each row (their 8 bits fit f16's
+// 11), which the softmax's factor takes back.
 #include "common.cuh"
 #include "decode.h"
 #include "per_device.h"
@@ -34,7 +44,6 @@ namespace pkc {
 
 namespace {
 
-constexpr int kRows = 16;
 constexpr int kStages = 3;  // tiles in a warp's ring
 constexpr int kSms = 148;
 
@@ -50,6 +59,13 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 8x8 matrix of 16-bit elements, transposed across the warp
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 
 // two e4m3 codes (the low or high half of w) -> f16x2
@@ -90,7 +106,7 @@ __device__ __forceinline__ int visible(const Item& it, int i) {
   return Q8 ? it.len - it.n + i + 1 : it.len;
 }
 
-// index of the 16-row block of partials
+// index of a block of rows
 __device__ __forceinline__ long long part_at(const DecodeAttnArgs& a, int row_tiles, int b, int h, int rt) {
   return ((long long)b * a.n_kv_heads + h) * row_tiles + rt;
 }
@@ -130,14 +146,15 @@ struct RowsLayout {
 };
 
 // H: type of q and out; Q8: 8-bit cache, else keys and values of type H; W
-// warps share the CTA's part of the keys.
-template <typename H, bool Q8, int D, int WT, int W>
-__global__ void __launch_bounds__(32 * W, 8 / W) k_attn_rows(const DecodeAttnArgs a, int row_tiles, int n_split) {
+// warps share the CTA's part of the keys; NB blocks of 8 query rows.
+template <typename H, bool Q8, int D, int WT, int W, int NB>
+__global__ void __launch_bounds__(32 * W) k_attn_rows(const DecodeAttnArgs a, int row_tiles, int n_split) {
   using M = typename std::conditional<Q8, __half, H>::type;  // type of the products
   constexpr int RB = Q8 ? D : 2 * D;                         // bytes of a row
   constexpr int KC = RB / 64;                                // 16-byte reads of a key row, per thread
   constexpr int VW = RB / 32;                                // 32-bit words of a value row, per thread
-  constexpr int NT = D / 8;                                  // 8-column tiles of the output
+  constexpr int MT = D / 16;                                 // 16-row tiles of the output
+  constexpr int R = 8 * NB;                                  // query rows
   using L = RowsLayout<RB, WT>;
   extern __shared__ __align__(128) uint8_t smem[];
 
@@ -155,13 +172,14 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_attn_rows(const DecodeAttnArg
     if (threadIdx.x == 0) report_error(a.err, DEV_ERR_BAD_SHAPE);
     return;
   }
-  const int rows = it.n * G;
-  if (rt * kRows >= rows) return;
+  const int rows = it.n * G, row0 = rt * R;
+  if (row0 >= rows) return;
 
-  // ---- this warp's tiles: t_begin + warp, + W, ...
+  // ---- this warp's tiles: t0, t0 + W, ...
   // the last row's last key ends the walk
-  const int last = min(rows, (rt + 1) * kRows) - 1;
+  const int last = min(rows, row0 + R) - 1;
   const int vmax = max(0, visible<Q8>(it, last / G));
+  const int vmin = Q8 ? visible<Q8>(it, row0 / G) : vmax;  // every row sees these
   const int n_tiles = (vmax + WT - 1) / WT;
   const int per = (n_tiles + n_split - 1) / n_split;
   const int t0 = split * per + warp, t_end = min(n_tiles, (split + 1) * per);
@@ -208,17 +226,24 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_attn_rows(const DecodeAttnArg
         kp += k0 * kst;
         vp += k0 * vst;
       }
+// a lane copies chunk `ch` of rows r0, r0 + 512 / RB, ...
+      constexpr int RS = 512 / RB;
+      const int r0 = lane / (RB / 16), ch = lane % (RB / 16);
+      kp += r0 * kst + ch * 16;
+      vp += r0 * vst + ch * 16;
+      if (left >= WT && on) {
 #pragma unroll
-      for (int j = 0; j < L::kTile / 512; ++j) {
-        const int q = j * 32 + lane, r = q / (RB / 16), ch = q % (RB / 16);
-        const bool in = on && r < left;
-        cp_async16(dst + key_at<RB>(r, ch), kp + (in ? r : 0) * kst + ch * 16, in ? 16 : 0);
-      }
+        for (int j = 0; j < WT / RS; ++j) cp_async16(dst + key_at<RB>(r0 + j * RS, ch), kp + j * RS * kst, 16);
 #pragma unroll
-      for (int j = 0; j < L::kTile / 512; ++j) {
-        const int q = j * 32 + lane, r = q / (RB / 16), ch = q % (RB / 16);
-        const bool in = on && r < left;
-        cp_async16(dst + L::kTile + value_at<RB>(r, ch), vp + (in ? r : 0) * vst + ch * 16, in ? 16 : 0);
+        for (int j = 0; j < WT / RS; ++j)
+          cp_async16(dst + L::kTile + value_at<RB>(r0 + j * RS, ch), vp + j * RS * vst, 16);
+      } else {
+#pragma unroll
+        for (int j = 0; j < WT / RS; ++j) {
+          const bool in = on && r0 + j * RS < left;
+          cp_async16(dst + key_at<RB>(r0 + j * RS, ch), in ? kp + j * RS * kst : kp - r0 * kst, in ? 16 : 0);
+          cp_async16(dst + L::kTile + value_at<RB>(r0 + j * RS, ch), in ? vp + j * RS * vst : vp - r0 * vst, in ? 16 : 0);
+        }
       }
     }
     cp_commit();
@@ -233,23 +258,28 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_attn_rows(const DecodeAttnArg
     id_next = ids[kStages - 1];
   }
 
-  // ---- queries: rows g and g + 8 of the tile, in the key loads' order
-  uint32_t qf[D / 16][4];
-  float rs[2];
-  int vis[2];
+  // ---- queries: row g of each block of 8, in the key reads' order
+  uint32_t qf[NB][D / 16][2];
+  float rs[NB][2];  // softmax factors and visible keys of rows 2 c and 2 c + 1
+  int vis[NB][2];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int r = rt * kRows + g + 8 * e;
+  for (int nb = 0; nb < NB; ++nb) {
+    const int r = row0 + nb * 8 + g;
     const bool on = r < rows;
     const int i = on ? r / G : 0, hd = h * G + (on ? r % G : 0);
-    vis[e] = on ? visible<Q8>(it, i) : 0;
     const H* qp = reinterpret_cast<const H*>(a.q) + (long long)(it.q0 + i) * a.ldq + hd * D;
-    rs[e] = a.scale_log2;
+    float factor = fabsf(a.scale_log2);
     uint4 w[D / 32];
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
       const int col = Q8 ? (j >> 1) * 64 + c * 16 + (j & 1) * 8 : j * 32 + c * 8;
       w[j] = on ? *reinterpret_cast<const uint4*>(qp + col) : make_uint4(0, 0, 0, 0);
+      if (a.scale_log2 < 0.f) {  // the factor stays positive: the largest product has the largest score
+        w[j].x ^= 0x80008000u;
+        w[j].y ^= 0x80008000u;
+        w[j].z ^= 0x80008000u;
+        w[j].w ^= 0x80008000u;
+      }
     }
     if constexpr (Q8 && is_bf16<H>::value) {
       float m = 0.f;
@@ -265,7 +295,7 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_attn_rows(const DecodeAttnArg
       // infinities as they are)
       const int x = ((__float_as_int(m) >> 23) & 255) - 127;
       const float f = m > 0.f && x < 127 && x > -126 ? __int_as_float((127 - x) << 23) : 1.f;
-      rs[e] /= f;
+      factor /= f;
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) {
         H* y = reinterpret_cast<H*>(&w[j]);
@@ -277,18 +307,29 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_attn_rows(const DecodeAttnArg
     }
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
-      qf[2 * j][e] = w[j].x;
-      qf[2 * j][2 + e] = w[j].y;
-      qf[2 * j + 1][e] = w[j].z;
-      qf[2 * j + 1][2 + e] = w[j].w;
+      qf[nb][2 * j][0] = w[j].x;
+      qf[nb][2 * j][1] = w[j].y;
+      qf[nb][2 * j + 1][0] = w[j].z;
+      qf[nb][2 * j + 1][1] = w[j].w;
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      rs[nb][x] = __shfl_sync(0xffffffffu, factor, 8 * c + 4 * x);
+      const int rr = row0 + nb * 8 + 2 * c + x;
+      vis[nb][x] = rr < rows ? visible<Q8>(it, rr / G) : 0;
     }
   }
-  float o[NT][4];
+
+  float o[NB][MT][4];
+  float m[NB][2], l[NB][2];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+  for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int i = 0; i < MT; ++i) o[nb][i][0] = o[nb][i][1] = o[nb][i][2] = o[nb][i][3] = 0.f;
+    m[nb][0] = m[nb][1] = -INFINITY;
+    l[nb][0] = l[nb][1] = 0.f;
+  }
+  float ref = -1000.f;  // the output is kept in units of 2^ref (8-bit cache)
 
   for (int i = 0; i < cnt; ++i) {
     cp_wait<kStages - 2>();
@@ -298,194 +339,289 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_attn_rows(const DecodeAttnArg
     const int k0 = (t0 + W * i) * WT;
     const uint8_t* kt = ring + (i % kStages) * L::kStage;
     const uint8_t* vt = kt + L::kTile;
-    float ks = 1.f, vs = 1.f;
+    float ks = 1.f, vs = 1.f, dv = 0.f;
+    bool apart = false;
     if constexpr (Q8) {
-      const float* sc = reinterpret_cast<const float*>(ring + kStages * L::kStage + (i % kStages) * 16);
-      ks = sc[0];
-      vs = sc[1];
+      const float2 sc = *reinterpret_cast<const float2*>(ring + kStages * L::kStage + (i % kStages) * 16);
+      ks = sc.x;
+      vs = sc.y;
       if (ks < 0.f) continue;
-    }
-    // ---- scores
-    float s[WT / 8][4];
+      const float ev = (float)((__float_as_int(vs) >> 23) - 127);
+      if (ev > ref) {
+        if (ref > -1000.f) {
+          const float f = ex2_approx(ref - ev);
 #pragma unroll
-    for (int i = 0; i < WT / 8; ++i) {
-      s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nb][j][e] *= f;
+        }
+        ref = ev;
+      }
+      dv = ev - ref;
+      apart = dv < -4.f;
+      if (apart) dv = 0.f;
+    }
+    // ---- scores: keys 16 t + g (and + 8) by rows 2 c, 2 c + 1
+    float s[NB][WT / 16][4];
+#pragma unroll
+    for (int t = 0; t < WT / 16; ++t) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) s[nb][t][0] = s[nb][t][1] = s[nb][t][2] = s[nb][t][3] = 0.f;
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
-        const uint4 kr = *reinterpret_cast<const uint4*>(kt + key_at<RB>(8 * i + g, 4 * j + c));
-        const uint32_t w[4] = {kr.x, kr.y, kr.z, kr.w};
+        const uint4 ka = *reinterpret_cast<const uint4*>(kt + key_at<RB>(16 * t + g, 4 * j + c));
+        const uint4 kb = *reinterpret_cast<const uint4*>(kt + key_at<RB>(16 * t + 8 + g, 4 * j + c));
+        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
         if constexpr (Q8) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) mma16816<M>(s[i], qf[4 * j + u], e4m3_lo(w[u]), e4m3_hi(w[u]));
+          for (int u = 0; u < 4; ++u) {
+            const uint32_t f[4] = {e4m3_lo(wa[u]), e4m3_lo(wb[u]), e4m3_hi(wa[u]), e4m3_hi(wb[u])};
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) mma16816<M>(s[nb][t], f, qf[nb][4 * j + u][0], qf[nb][4 * j + u][1]);
+          }
         } else {
-          mma16816<M>(s[i], qf[2 * j], w[0], w[1]);
-          mma16816<M>(s[i], qf[2 * j + 1], w[2], w[3]);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t f[4] = {wa[2 * u], wb[2 * u], wa[2 * u + 1], wb[2 * u + 1]};
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) mma16816<M>(s[nb][t], f, qf[nb][2 * j + u][0], qf[nb][2 * j + u][1]);
+          }
         }
       }
     }
     // ---- running softmax in the log2 domain
-    float mt[2] = {-INFINITY, -INFINITY};
+    const bool partial = k0 + WT > vmin;  // some row does not see every key of the tile
+    if (partial) {
 #pragma unroll
-    for (int i = 0; i < WT / 8; ++i)
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = k0 + 8 * i + 2 * c + (e & 1);
-        s[i][e] = key < vis[e >> 1] ? s[i][e] * (rs[e >> 1] * ks) : -INFINITY;
-        mt[e >> 1] = fmaxf(mt[e >> 1], s[i][e]);
+        for (int t = 0; t < WT / 16; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (k0 + 16 * t + g + 8 * (e >> 1) >= vis[nb][e & 1]) s[nb][t][e] = -INFINITY;
+    }
+    uint32_t pf[NB][WT / 16][2];
+    float mu[NB][2], alpha[NB][2];
+    bool moved = false;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float mt[2] = {s[nb][0][0], s[nb][0][1]};
+#pragma unroll
+      for (int t = 0; t < WT / 16; ++t) {
+        mt[0] = fmaxf(mt[0], fmaxf(s[nb][t][0], s[nb][t][2]));
+        mt[1] = fmaxf(mt[1], fmaxf(s[nb][t][1], s[nb][t][3]));
       }
-    float mu[2], alpha[2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], 1));
-      mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], 2));
-      const float mn = fmaxf(m[e], mt[e]);
-      mu[e] = mn == -INFINITY ? 0.f : mn;
-      alpha[e] = ex2_approx(m[e] - mu[e]);
-      m[e] = mn;
-      l[e] *= alpha[e];
-    }
-    if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+      for (int x = 0; x < 2; ++x) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] *= alpha[e >> 1];
-    }
-    uint32_t pf[WT / 16][4];
-#pragma unroll
-    for (int i = 0; i < WT / 8; ++i) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[i][e] = ex2_approx(s[i][e] - mu[e >> 1]);
-        l[e >> 1] += s[i][e];
+        for (int k = 4; k < 32; k <<= 1) mt[x] = fmaxf(mt[x], __shfl_xor_sync(0xffffffffu, mt[x], k));
+        const float mn = fmaxf(m[nb][x], mt[x] * (rs[nb][x] * ks));  // (a NaN of no key and no factor is passed over)
+        mu[nb][x] = mn == -INFINITY ? 0.f : mn;
+        alpha[nb][x] = ex2_approx(m[nb][x] - mu[nb][x]);
+        m[nb][x] = mn;
+        moved |= alpha[nb][x] != 1.f;
       }
-      // probabilities in the products' type: at most half a step off each
-      pf[i >> 1][2 * (i & 1)] = pack2<M>(s[i][0], s[i][1]);
-      pf[i >> 1][2 * (i & 1) + 1] = pack2<M>(s[i][2], s[i][3]);
     }
-    // ---- values: keys 16 i + {0, 1, 8, 9} + 2 c
-    uint32_t vr[WT / 4][VW];
+    if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-    for (int i = 0; i < WT / 4; ++i) {
-      const int r = 16 * (i >> 2) + 2 * c + (i & 1) + 8 * ((i >> 1) & 1);
-      if constexpr (VW == 2) {
-        const uint2 x = *reinterpret_cast<const uint2*>(vt + value_at<RB>(r, g >> 1) + (g & 1) * 8);
-        vr[i][0] = x.x;
-        vr[i][1] = x.y;
-      } else {
+      for (int nb = 0; nb < NB; ++nb) {
+        l[nb][0] *= alpha[nb][0];
+        l[nb][1] *= alpha[nb][1];
 #pragma unroll
-        for (int j = 0; j < VW / 4; ++j) {
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nb][j][e] *= alpha[nb][e & 1];
+      }
+    }
+    const float back = Q8 ? ex2_approx(-dv) : 1.f;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const float f0 = rs[nb][0] * ks, f1 = rs[nb][1] * ks, z0 = dv - mu[nb][0], z1 = dv - mu[nb][1];
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < WT / 16; ++t) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = ex2_approx(fmaf(s[nb][t][e], e & 1 ? f1 : f0, e & 1 ? z1 : z0));
+        if (partial) {  // (zero also where the factor is zero)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (k0 + 16 * t + g + 8 * (e >> 1) >= vis[nb][e & 1]) p[e] = 0.f;
+        }
+        sum[0] += p[0] + p[2];
+        sum[1] += p[1] + p[3];
+        // probabilities in the products' type: at most half a step off each
+        pf[nb][t][0] = movmatrix(pack2<M>(p[0], p[1]));
+        pf[nb][t][1] = movmatrix(pack2<M>(p[2], p[3]));
+      }
+      l[nb][0] = fmaf(sum[0], back, l[nb][0]);
+      l[nb][1] = fmaf(sum[1], back, l[nb][1]);
+    }
+    // ---- values: keys 16 t + {0, 1, 8, 9} + 2 c; word w of a row holds the
+    // columns of output tile w (16-bit) or tiles 2 w, 2 w + 1 (8-bit)
+    constexpr int VC = VW == 2 ? 2 : 4;  // words of one read
+#pragma unroll
+    for (int j = 0; j < VW / VC; ++j) {
+      uint32_t vr[WT / 4][VC];
+#pragma unroll
+      for (int k = 0; k < WT / 4; ++k) {
+        const int r = 16 * (k >> 2) + 2 * c + (k & 1) + 8 * ((k >> 1) & 1);
+        if constexpr (VC == 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(vt + value_at<RB>(r, g >> 1) + (g & 1) * 8);
+          vr[k][0] = x.x;
+          vr[k][1] = x.y;
+        } else {
           const uint4 x = *reinterpret_cast<const uint4*>(vt + value_at<RB>(r, 8 * j + g));
-          vr[i][4 * j] = x.x;
-          vr[i][4 * j + 1] = x.y;
-          vr[i][4 * j + 2] = x.z;
-          vr[i][4 * j + 3] = x.w;
+          vr[k][0] = x.x;
+          vr[k][1] = x.y;
+          vr[k][2] = x.z;
+          vr[k][3] = x.w;
         }
       }
-    }
-    if constexpr (Q8) {
-#pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        float acc[4][4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) acc[x][0] = acc[x][1] = acc[x][2] = acc[x][3] = 0.f;
-#pragma unroll
-        for (int i = 0; i < WT / 16; ++i) {
-          const uint32_t a0 = vr[4 * i][w], a1 = vr[4 * i + 1][w], a2 = vr[4 * i + 2][w], a3 = vr[4 * i + 3][w];
-          const uint32_t p0 = __byte_perm(a0, a1, 0x5140), p1 = __byte_perm(a2, a3, 0x5140);
-          const uint32_t p2 = __byte_perm(a0, a1, 0x7362), p3 = __byte_perm(a2, a3, 0x7362);
-          mma16816<M>(acc[0], pf[i], e4m3_lo(p0), e4m3_lo(p1));
-          mma16816<M>(acc[1], pf[i], e4m3_hi(p0), e4m3_hi(p1));
-          mma16816<M>(acc[2], pf[i], e4m3_lo(p2), e4m3_lo(p3));
-          mma16816<M>(acc[3], pf[i], e4m3_hi(p2), e4m3_hi(p3));
+      auto product = [&](float (&acc)[NB][4], int w, int half, int t) {
+        const uint32_t a0 = vr[4 * t][w], a1 = vr[4 * t + 1][w], a2 = vr[4 * t + 2][w], a3 = vr[4 * t + 3][w];
+        uint32_t f[4];
+        if constexpr (Q8) {
+          const uint32_t sel = half ? 0x7362 : 0x5140;
+          const uint32_t lo = __byte_perm(a0, a1, sel), hi = __byte_perm(a2, a3, sel);
+          f[0] = e4m3_lo(lo);
+          f[1] = e4m3_hi(lo);
+          f[2] = e4m3_lo(hi);
+          f[3] = e4m3_hi(hi);
+        } else {
+          f[0] = __byte_perm(a0, a1, 0x5410);
+          f[1] = __byte_perm(a0, a1, 0x7632);
+          f[2] = __byte_perm(a2, a3, 0x5410);
+          f[3] = __byte_perm(a2, a3, 0x7632);
         }
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int nb = 0; nb < NB; ++nb) mma16816<M>(acc[nb], f, pf[nb][t][0], pf[nb][t][1]);
+      };
+      constexpr int HV = Q8 ? 2 : 1;
+      if (!apart) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[4 * w + x][e] = fmaf(acc[x][e], vs, o[4 * w + x][e]);
+        for (int w = 0; w < VC; ++w)
+#pragma unroll
+          for (int half = 0; half < HV; ++half) {
+            const int tile = (j * VC + w) * HV + half;
+            float acc[NB][4];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[nb][e] = o[nb][tile][e];
+#pragma unroll
+            for (int t = 0; t < WT / 16; ++t) product(acc, w, half, t);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nb][tile][e] = acc[nb][e];
+          }
+      } else if constexpr (Q8) {
+        const float f = ex2_approx((float)((__float_as_int(vs) >> 23) - 127) - ref);
+#pragma unroll
+        for (int w = 0; w < VC; ++w)
+#pragma unroll
+          for (int half = 0; half < HV; ++half) {
+            const int tile = (j * VC + w) * HV + half;
+            float acc[NB][4] = {};
+#pragma unroll
+            for (int t = 0; t < WT / 16; ++t) product(acc, w, half, t);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nb][tile][e] = fmaf(acc[nb][e], f, o[nb][tile][e]);
+          }
       }
-    } else {
-#pragma unroll
-      for (int w = 0; w < VW; ++w)
-#pragma unroll
-        for (int i = 0; i < WT / 16; ++i) {
-          const uint32_t a0 = vr[4 * i][w], a1 = vr[4 * i + 1][w], a2 = vr[4 * i + 2][w], a3 = vr[4 * i + 3][w];
-          mma16816<M>(o[2 * w], pf[i], __byte_perm(a0, a1, 0x5410), __byte_perm(a2, a3, 0x5410));
-          mma16816<M>(o[2 * w + 1], pf[i], __byte_perm(a0, a1, 0x7632), __byte_perm(a2, a3, 0x7632));
-        }
     }
+  }
+  if constexpr (Q8) {
+    const float f = ref > -1000.f ? ex2_approx(ref) : 0.f;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nb][j][e] *= f;
   }
 
-  // ---- what this warp holds of rows g (e = 0) and g + 8: four columns at a time
+  // ---- what this warp holds: rows 2 c and 2 c + 1 of each block of 8, four
+  // neighbouring columns at a time
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-  }
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int k = 4; k < 32; k <<= 1) l[nb][x] += __shfl_xor_sync(0xffffffffu, l[nb][x], k);
   auto each = [&](auto&& f) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)  // column 2 c + n of the 8-column tiles
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int i = 0; i < NT; i += 4) {
-          const int dim = Q8 ? (2 * c + n) * (D / 8) + i : (i >> 3) * 64 + (2 * c + n) * 8 + (i & 7);
-          const int x = 2 * e + n;
-          f(e, dim, make_float4(o[i][x], o[i + 1][x], o[i + 2][x], o[i + 3][x]));
+        for (int i = 0; i < MT; i += 2) {
+          const int dim = Q8 ? g * (D / 8) + 2 * i : (i >> 2) * 64 + g * 8 + 2 * (i & 3);
+          f(nb, x, dim, make_float4(o[nb][i][x], o[nb][i][2 + x], o[nb][i + 1][x], o[nb][i + 1][2 + x]));
         }
   };
-  const int valid = min(kRows, rows - rt * kRows);
-  float* po = a.ws + (part_at(a, row_tiles, b, h, rt) * n_split + split) * (kRows * (D + 2));
+  const int valid = min(R, rows - row0);
+  float* po = a.ws + (part_at(a, row_tiles, b, h, rt) * n_split + split) * (R * (D + 2));
   auto store_out = [&](int r, int dim, float4 v) {
-    const int row = rt * kRows + r;
+    const int row = row0 + r;
     H* op = reinterpret_cast<H*>(a.out) + (long long)(it.q0 + row / G) * a.ldo + (h * G + row % G) * D + dim;
     *reinterpret_cast<uint2*>(op) = make_uint2(pack2<H>(v.x, v.y), pack2<H>(v.z, v.w));
   };
   if constexpr (W == 1) {
     if (n_split == 1) {
-      float inv[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) inv[e] = l[e] == 0.f ? 0.f : 1.f / l[e];  // no key seen: zeros
-      each([&](int e, int dim, float4 v) {
-        if (g + 8 * e < valid)
-          store_out(g + 8 * e, dim, make_float4(v.x * inv[e], v.y * inv[e], v.z * inv[e], v.w * inv[e]));
+      each([&](int nb, int x, int dim, float4 v) {
+        const int r = nb * 8 + 2 * c + x;
+        const float inv = l[nb][x] == 0.f ? 0.f : 1.f / l[nb][x];  // no key seen: zeros
+        if (r < valid) store_out(r, dim, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
       });
     } else {
-      each([&](int e, int dim, float4 v) {
-        if (g + 8 * e < valid) *reinterpret_cast<float4*>(po + (g + 8 * e) * D + dim) = v;
+      each([&](int nb, int x, int dim, float4 v) {
+        const int r = nb * 8 + 2 * c + x;
+        if (r < valid) *reinterpret_cast<float4*>(po + r * D + dim) = v;
       });
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (c == 0 && g + 8 * e < valid)
-          *reinterpret_cast<float2*>(po + kRows * D + 2 * (g + 8 * e)) = make_float2(m[e], l[e]);
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int r = nb * 8 + 2 * c + x;
+          if (g == 0 && r < valid) *reinterpret_cast<float2*>(po + R * D + 2 * r) = make_float2(m[nb][x], l[nb][x]);
+        }
     }
   } else {
     // ---- join the warps, in the rings' memory
     cp_wait<0>();
     __syncthreads();
     constexpr int LD = D + 4;
-    float* s_o = reinterpret_cast<float*>(smem);          // [W][kRows][LD]
-    float* s_ml = s_o + W * kRows * LD;                   // [W][kRows][2]
-    static_assert((W * kRows * (LD + 2)) * 4 <= W * L::kWarp, "the join fits the rings");
-    each([&](int e, int dim, float4 v) {
-      *reinterpret_cast<float4*>(s_o + (warp * kRows + g + 8 * e) * LD + dim) = v;
+    float* s_o = reinterpret_cast<float*>(smem);  // [W][R][LD]
+    float* s_ml = s_o + W * R * LD;               // [W][R][2]
+    static_assert((W * R * (LD + 2)) * 4 <= W * L::kWarp, "the join fits the rings");
+    each([&](int nb, int x, int dim, float4 v) {
+      *reinterpret_cast<float4*>(s_o + (warp * R + nb * 8 + 2 * c + x) * LD + dim) = v;
     });
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (c == 0)
-        *reinterpret_cast<float2*>(s_ml + (warp * kRows + g + 8 * e) * 2) = make_float2(m[e], l[e]);
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (g == 0)
+          *reinterpret_cast<float2*>(s_ml + (warp * R + nb * 8 + 2 * c + x) * 2) = make_float2(m[nb][x], l[nb][x]);
     __syncthreads();
     for (int idx = threadIdx.x; idx < valid * (D / 4); idx += 32 * W) {
       const int r = idx / (D / 4), d4 = idx % (D / 4) * 4;
       float mm = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < W; ++w) mm = fmaxf(mm, s_ml[(w * kRows + r) * 2]);
+      for (int w = 0; w < W; ++w) mm = fmaxf(mm, s_ml[(w * R + r) * 2]);
       const float base = mm == -INFINITY ? 0.f : mm;
       float ll = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const float f = ex2_approx(s_ml[(w * kRows + r) * 2] - base);
-        ll += s_ml[(w * kRows + r) * 2 + 1] * f;
-        const float4 v = *reinterpret_cast<const float4*>(s_o + (w * kRows + r) * LD + d4);
+        const float f = ex2_approx(s_ml[(w * R + r) * 2] - base);
+        ll += s_ml[(w * R + r) * 2 + 1] * f;
+        const float4 v = *reinterpret_cast<const float4*>(s_o + (w * R + r) * LD + d4);
         x[0] = fmaf(v.x, f, x[0]);
         x[1] = fmaf(v.y, f, x[1]);
         x[2] = fmaf(v.z, f, x[2]);
@@ -496,17 +632,21 @@ __global__ void __launch_bounds__(32 * W, 8 / W) k_attn_rows(const DecodeAttnArg
         store_out(r, d4, make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv));
       } else {
         *reinterpret_cast<float4*>(po + r * D + d4) = make_float4(x[0], x[1], x[2], x[3]);
-        if (d4 == 0) *reinterpret_cast<float2*>(po + kRows * D + 2 * r) = make_float2(mm, ll);
+        if (d4 == 0) *reinterpret_cast<float2*>(po + R * D + 2 * r) = make_float2(mm, ll);
       }
     }
   }
 }
 
-// Joins the parts of one 16-row block: o = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).
-template <typename H, bool Q8, int D>
-__global__ void __launch_bounds__(kRows * D / 4) k_attn_join(const DecodeAttnArgs a, int row_tiles, int n_split) {
+// Joins the parts of one row: o = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).
+// Four warps take every fourth part each (a part is a read that depends on
+// nothing), then add up.
+template <typename H, bool Q8, int D, int R>
+__global__ void __launch_bounds__(128) k_attn_join(const DecodeAttnArgs a, int row_tiles, int n_split) {
+  __shared__ float s_x[4][D], s_l[4];
   const int G = a.n_heads / a.n_kv_heads;
-  int rest = blockIdx.x;
+  const int r = blockIdx.x % R;
+  int rest = blockIdx.x / R;
   const int rt = rest % row_tiles;
   rest /= row_tiles;
   const int h = rest % a.n_kv_heads, b = rest / a.n_kv_heads;
@@ -514,71 +654,93 @@ __global__ void __launch_bounds__(kRows * D / 4) k_attn_join(const DecodeAttnArg
   pdl_trigger();
   const Item it = load_item<Q8>(a, b);
   if (!it.ok) return;
-  const int rows = it.n * G, r = threadIdx.x / (D / 4), d4 = threadIdx.x % (D / 4) * 4, row = rt * kRows + r;
-  if (row >= rows) return;
-  const float* p = a.ws + part_at(a, row_tiles, b, h, rt) * n_split * (kRows * (D + 2));
-  float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < n_split; ++s, p += kRows * (D + 2)) {
-    const float ms = p[kRows * D + 2 * r], ls = p[kRows * D + 2 * r + 1];
-    if (ls == 0.f) continue;  // a part without keys
-    const float4 v = *reinterpret_cast<const float4*>(p + r * D + d4);
-    const float mn = fmaxf(m, ms), f0 = ex2_approx(m - mn), f1 = ex2_approx(ms - mn);
-    l = l * f0 + ls * f1;
-    x[0] = x[0] * f0 + v.x * f1;
-    x[1] = x[1] * f0 + v.y * f1;
-    x[2] = x[2] * f0 + v.z * f1;
-    x[3] = x[3] * f0 + v.w * f1;
-    m = mn;
+  const int row = rt * R + r, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (row >= it.n * G) return;
+  constexpr int PS = R * (D + 2);  // floats of a part
+  const float* p = a.ws + part_at(a, row_tiles, b, h, rt) * n_split * PS;
+  // the largest maximum (n_split <= 64: two parts a lane)
+  float m = -INFINITY;
+  for (int s = lane; s < n_split; s += 32) m = fmaxf(m, p[s * PS + R * D + 2 * r]);
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+  const float base = m == -INFINITY ? 0.f : m;
+  constexpr int V = D / 32;  // columns of a lane
+  float x[V] = {}, l = 0.f;
+#pragma unroll 4
+  for (int s = warp; s < n_split; s += 4) {
+    const float2 ml = *reinterpret_cast<const float2*>(p + s * PS + R * D + 2 * r);
+    const float f = ex2_approx(ml.x - base);
+    l = fmaf(ml.y, f, l);
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = fmaf(p[s * PS + r * D + v * 32 + lane], f, x[v]);
   }
+#pragma unroll
+  for (int v = 0; v < V; ++v) s_x[warp][v * 32 + lane] = x[v];
+  if (lane == 0) s_l[warp] = l;
+  __syncthreads();
+  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  H* op = reinterpret_cast<H*>(a.out) + (long long)(it.q0 + row / G) * a.ldo + (h * G + row % G) * D + d4;
-  *reinterpret_cast<uint2*>(op) = make_uint2(pack2<H>(x[0] * inv, x[1] * inv), pack2<H>(x[2] * inv, x[3] * inv));
+  if (threadIdx.x < D / 2) {
+    const int d = 2 * threadIdx.x;
+    const float y0 = (s_x[0][d] + s_x[1][d]) + (s_x[2][d] + s_x[3][d]);
+    const float y1 = (s_x[0][d + 1] + s_x[1][d + 1]) + (s_x[2][d + 1] + s_x[3][d + 1]);
+    H* op = reinterpret_cast<H*>(a.out) + (long long)(it.q0 + row / G) * a.ldo + (h * G + row % G) * D + d;
+    *reinterpret_cast<uint32_t*>(op) = pack2<H>(y0 * inv, y1 * inv);
+  }
 }
 
-// How a call is cut: `warps` a CTA and parts of each item's keys.
-//  - Many blocks of rows: a warp takes one alone (CTAs of one warp, no join).
+// How a call is cut.
+//  - Blocks of 8 rows, or of 16 where an item has more: they share one read of
+//    the keys.
+//  - Many blocks: a warp takes one alone (CTAs of one warp, no join).
 //  - Else four warps share a part, and the keys are cut into as many parts as
 //    give about six CTAs an SM (lengths differ; two run at a time), of at
 //    least 128 keys.
 struct Plan {
-  int warps, n_split;
+  int rows, row_tiles, warps, n_split;
+  long long blocks;
 };
-Plan plan_rows(long long blocks, int max_kv) {
-  if (blocks >= 8LL * kSms) return {1, 1};
-  const long long want = (6LL * kSms + blocks - 1) / blocks;
-  const long long most = (max_kv + 127) / 128;
-  const long long n = want < most ? want : most;
-  return {4, n < 1 ? 1 : n > 64 ? 64 : (int)n};
+Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads) {
+  Plan p;
+  const long long rows = (long long)max_q * (n_heads / n_kv_heads);
+  p.rows = rows <= 8 ? 8 : 16;
+  p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
+  p.blocks = (long long)n_items * n_kv_heads * p.row_tiles;
+  p.warps = 1;
+  p.n_split = 1;
+  if (p.blocks < 8LL * kSms) {
+    p.warps = 4;
+    const long long want = (6LL * kSms + p.blocks - 1) / (p.blocks > 0 ? p.blocks : 1);
+    const long long most = (max_kv + 127) / 128;
+    const long long n = want < most ? want : most;
+    p.n_split = n < 1 ? 1 : n > 64 ? 64 : (int)n;
+  }
+  return p;
 }
 
-long long row_blocks(int n_items, int max_q, int n_heads, int n_kv_heads, int* row_tiles) {
-  *row_tiles = (int)(((long long)max_q * (n_heads / n_kv_heads) + kRows - 1) / kRows);
-  return (long long)n_items * n_kv_heads * *row_tiles;
-}
-
-template <typename H, bool Q8, int D, int WT, int W>
-cudaError_t launch_w(const DecodeAttnArgs& a, long long blocks, int rt, int n_split, cudaStream_t st) {
-  auto kern = k_attn_rows<H, Q8, D, WT, W>;
+template <typename H, bool Q8, int D, int WT, int W, int NB>
+cudaError_t launch_w(const DecodeAttnArgs& a, const Plan& p, cudaStream_t st) {
+  auto kern = k_attn_rows<H, Q8, D, WT, W, NB>;
   constexpr int smem = W * RowsLayout<Q8 ? D : 2 * D, WT>::kWarp;
   static PerDevice once;
   int unused = 0;
-  const cudaError_t e = per_device(once, &unused, [&](int, int&) {
+  cudaError_t e = per_device(once, &unused, [&](int, int&) {
     return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (e != cudaSuccess) return e;
-  return launch_pdl(kern, dim3((unsigned)(blocks * n_split)), dim3(32 * W), smem, st, a, rt, n_split);
+  e = launch_pdl(kern, dim3((unsigned)(p.blocks * p.n_split)), dim3(32 * W), smem, st, a, p.row_tiles, p.n_split);
+  if (e != cudaSuccess || p.n_split == 1) return e;
+  return launch_pdl(k_attn_join<H, Q8, D, 8 * NB>, dim3((unsigned)(p.blocks * 8 * NB)), dim3(128), 0, st, a, p.row_tiles,
+                    p.n_split);
 }
 
 template <typename H, bool Q8, int D, int WT>
 cudaError_t launch_rows(const DecodeAttnArgs& a, cudaStream_t st) {
-  int rt = 0;
-  const long long blocks = row_blocks(a.n_items, a.max_q, a.n_heads, a.n_kv_heads, &rt);
-  const Plan p = plan_rows(blocks, a.max_kv);
-  if (blocks * p.n_split > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const cudaError_t e = p.warps == 1 ? launch_w<H, Q8, D, WT, 1>(a, blocks, rt, p.n_split, st)
-                                     : launch_w<H, Q8, D, WT, 4>(a, blocks, rt, p.n_split, st);
-  if (e != cudaSuccess || p.n_split == 1) return e;
-  return launch_pdl(k_attn_join<H, Q8, D>, dim3((unsigned)blocks), dim3(kRows * D / 4), 0, st, a, rt, p.n_split);
+  const Plan p = plan_rows(a.n_items, a.max_q, a.max_kv, a.n_heads, a.n_kv_heads);
+  if (p.blocks * p.n_split * 16 > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (p.rows == 8)
+    return p.warps == 1 ? launch_w<H, Q8, D, WT, 1, 1>(a, p, st) : launch_w<H, Q8, D, WT, 4, 1>(a, p, st);
+  return p.warps == 1 ? launch_w<H, Q8, D, WT, 1, 2>(a, p, st) : launch_w<H, Q8, D, WT, 4, 2>(a, p, st);
 }
 
 template <typename H>
@@ -593,12 +755,9 @@ cudaError_t launch_h(const DecodeAttnArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-size_t decode_attn_ws_bytes(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, int head_dim, bool q8) {
-  int rt = 0;
-  const long long blocks = row_blocks(n_items, max_q, n_heads, n_kv_heads, &rt);
-  if (blocks <= 0) return 0;
-  const int n_split = plan_rows(blocks, max_kv).n_split;
-  return n_split == 1 ? 0 : (size_t)blocks * n_split * kRows * (head_dim + 2) * sizeof(float);
+size_t decode_attn_ws_bytes(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, int head_dim, bool) {
+  const Plan p = plan_rows(n_items, max_q, max_kv, n_heads, n_kv_heads);
+  return p.n_split == 1 ? 0 : (size_t)p.blocks * p.n_split * p.rows * (head_dim + 2) * sizeof(float);
 }
 
 cudaError_t decode_attn_launch(const DecodeAttnArgs& a, bool bf16, cudaStream_t st) {
