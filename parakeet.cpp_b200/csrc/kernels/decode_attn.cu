@@ -8,7 +8,7 @@
 // bound by memory: one CTA takes up to 16 rows (tokens x heads of one shared
 // key head) of one item and one part of its keys; its warps walk tiles of WT
 // keys on their own, each with its own ring of tiles in shared memory (filled
-// by cp.async two tiles ahead, no barrier but the warp's own) and its own
+// by cp.async ahead of its use, no barrier but the warp's own) and its own
 // running maximum and sum. Parts are joined by k_attn_join when there is more
 // than one.
 //
@@ -44,7 +44,6 @@ namespace pkc {
 
 namespace {
 
-constexpr int kStages = 3;  // tiles in a warp's ring
 constexpr int kSms = 148;
 
 template <typename M>
@@ -138,8 +137,14 @@ __device__ __forceinline__ int value_at(int r, int ch) {
 
 // Shared memory of a CTA of W warps: the rings, then each stage's two scales;
 // the join of the warps reuses the rings.
-template <int RB, int WT>
+//
+// Two tiles a ring and 168 registers let twelve warps run on an SM, which is
+// what hides the latencies here (three tiles and eight warps: long contexts 68
+// instead of XX us); with two blocks of rows the registers leave eight, and
+// three tiles.
+template <int RB, int WT, int NB>
 struct RowsLayout {
+  static constexpr int kStages = NB == 1 ? 2 : 3;
   static constexpr int kTile = WT * RB;  // keys or values of a tile
   static constexpr int kStage = 2 * kTile;
   static constexpr int kWarp = kStages * kStage + kStages * 16;  // + {key scale, value scale}
@@ -148,14 +153,15 @@ struct RowsLayout {
 // H: type of q and out; Q8: 8-bit cache, else keys and values of type H; W
 // warps share the CTA's part of the keys; NB blocks of 8 query rows.
 template <typename H, bool Q8, int D, int WT, int W, int NB>
-__global__ void __launch_bounds__(32 * W) k_attn_rows(const DecodeAttnArgs a, int row_tiles, int n_split) {
+__global__ void __launch_bounds__(32 * W, NB == 1 ? 12 / W : 8 / W) k_attn_rows(const DecodeAttnArgs a, int row_tiles, int n_split) {
   using M = typename std::conditional<Q8, __half, H>::type;  // type of the products
   constexpr int RB = Q8 ? D : 2 * D;                         // bytes of a row
   constexpr int KC = RB / 64;                                // 16-byte reads of a key row, per thread
   constexpr int VW = RB / 32;                                // 32-bit words of a value row, per thread
   constexpr int MT = D / 16;                                 // 16-row tiles of the output
   constexpr int R = 8 * NB;                                  // query rows
-  using L = RowsLayout<RB, WT>;
+  using L = RowsLayout<RB, WT, NB>;
+  constexpr int kStages = L::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
 
   const int G = a.n_heads / a.n_kv_heads;
@@ -721,7 +727,7 @@ Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads) 
 template <typename H, bool Q8, int D, int WT, int W, int NB>
 cudaError_t launch_w(const DecodeAttnArgs& a, const Plan& p, cudaStream_t st) {
   auto kern = k_attn_rows<H, Q8, D, WT, W, NB>;
-  constexpr int smem = W * RowsLayout<Q8 ? D : 2 * D, WT>::kWarp;
+  constexpr int smem = W * RowsLayout<Q8 ? D : 2 * D, WT, NB>::kWarp;
   static PerDevice once;
   int unused = 0;
   cudaError_t e = per_device(once, &unused, [&](int, int&) {
