@@ -42,8 +42,14 @@ pkc_status check_device(const char* what, void* stream, const void* const* ptrs,
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (st && st != cudaStreamLegacy && st != cudaStreamPerThread) {
-    int sdev = -1;
-    if (cudaStreamGetDevice(st, &sdev) != cudaSuccess) {
+    // (a capturing stream must not be asked for its device: that ends the capture)
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &cap) != cudaSuccess) {
+      cudaGetLastError();
+      return bad(what, "invalid stream");
+    }
+    int sdev = dev;
+    if (cap == cudaStreamCaptureStatusNone && cudaStreamGetDevice(st, &sdev) != cudaSuccess) {
       cudaGetLastError();
       return bad(what, "invalid stream");
     }
