@@ -9,24 +9,28 @@
 // that is NaN offer -inf.
 //
 // Within a row the order is that of the logits, so each CTA reads its row (or
-// its part of one) once and keeps the K largest as keys (ordered value bits
-// over the inverted index); only between rows do the sums matter. Those are
-// kept in f64 from groups of f32 exponentials, and the scores are compared in
-// f64: two hypotheses a few f32 steps apart come out in the order of their
-// exact scores. A cluster holds one item: its first CTA joins the rows' lists
-// through distributed shared memory, so there is one launch and no workspace.
+// its part of one) once from memory and keeps the K largest as keys (ordered
+// value bits over the inverted index); only between rows do the sums matter.
+// Those are kept in f64, and the scores are compared in f64: two hypotheses a few f32 steps apart come out in the order
+// of their exact scores. A cluster holds one item: its CTAs put their lists
+// into the first one's shared memory, which joins them, so there is one launch
+// and no workspace.
+//
+// The K largest: the first pass leaves each thread's largest value; each warp
+// sorts its lanes' and takes the K-th, a value that K elements reach; the
+// largest of these bounds leaves a few dozen candidates, which the second pass
+// (out of the L1 cache) gathers and which are put in order by counting. Where
+// ties leave too many of them, the keys are taken one after another.
 #include "common.cuh"
 #include "decode.h"
-#include "per_device.h"
 
 namespace pkc {
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 32;                    // elements of a block, per thread
-constexpr int kBlock = kThreads * kPer;     // elements that are looked at together
-constexpr int kCap = kMaxBeams * kPer + kMaxBeams;  // candidates of one block at most, see gather
+constexpr int kWarps = kThreads / 32;
+constexpr int kCap = 512;  // candidates at most
 constexpr int kMaxCluster = 8;
 
 // Larger keys for larger values, and for the lower index among equal values.
@@ -41,240 +45,317 @@ __device__ __forceinline__ float key_value(unsigned long long k) {
 }
 __device__ __forceinline__ int key_index(unsigned long long k) { return (int)(0xffffffffu - (unsigned int)k); }
 
-template <typename T>
-__device__ __forceinline__ float load_f(const T* p);
-template <>
-__device__ __forceinline__ float load_f<float>(const float* p) { return *p; }
-template <>
-__device__ __forceinline__ float load_f<__half>(const __half* p) { return __half2float(*p); }
-template <>
-__device__ __forceinline__ float load_f<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+// A thread's share of row[v0 .. v1): f(values, first index, how many, index
+// step) for VE elements at a time, missing ones -inf. Which thread takes which
+// element, and so the order of the sums, goes by the index alone and is the
+// same for every row of a call: equal rows have equal sums, to the bit, and tie.
+// Aligned: every row of the call starts on 16 bytes (v0 a multiple of VE).
+template <typename T, bool ALIGNED, typename F>
+__device__ __forceinline__ void each_group(const T* row, int v0, int v1, F&& f) {
+  constexpr int VE = 16 / sizeof(T);
+  auto value = [](T x) -> float {
+    if constexpr (sizeof(T) == 4)
+      return x;
+    else
+      return from_h(x);
+  };
+  if constexpr (ALIGNED) {
+#pragma unroll 4
+    for (int v = v0 + threadIdx.x * VE; v < v1; v += kThreads * VE) {
+      float x[VE];
+      const int n = min(VE, v1 - v);
+      if (n == VE) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(row + v);
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          if constexpr (sizeof(T) == 4) {
+            x[e] = __uint_as_float(w[e]);
+          } else {
+            const uint32_t u = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
+            x[e] = is_bf16<T>::value ? __uint_as_float(u << 16) : __half2float(__ushort_as_half((unsigned short)u));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x[e] = e < n ? value(row[v + e]) : -INFINITY;
+      }
+      f(x, v, n, 1);
+    }
+  } else {
+#pragma unroll 2
+    for (int v = v0 + threadIdx.x; v < v1; v += kThreads * VE) {
+      float x[VE];
+      const int n = min(VE, (v1 - v + kThreads - 1) / kThreads);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) x[e] = e < n ? value(row[v + e * kThreads]) : -INFINITY;
+      f(x, v, n, kThreads);
+    }
+  }
+}
 
 // What one part of one row gives: its K largest logits, in order, and the sum
 // of its exponentials.
 struct Part {
   unsigned long long key[kMaxBeams];
-  double sum;  // of exp(x - max); NaN where the part holds a NaN
+  double sum;  // of exp(x - max); NaN where the part holds a NaN or +inf
   float max;
   int n;       // keys
 };
 
 struct SelectShared {
-  Part part[kMaxBeams];  // this CTA's rows (one part each)
-  unsigned long long list[kCap];
-  unsigned long long best[kThreads];
-  double sum[kThreads / 32];
-  float max[kThreads / 32];
-  int count, nan;
-  unsigned long long thr;
+  Part part[kMaxBeams];  // in the cluster's first CTA: those of [row][part of it]
+  Part mine;
+  union {
+    unsigned long long list[kCap];
+    struct {
+      unsigned long long score[kMaxBeams * kMaxBeams];  // ordered bits of the candidates' scores
+      long long at[kMaxBeams * kMaxBeams];              // beam * V + token, or -1
+    } cand;
+  };
+  unsigned long long best[kMaxBeams];
+  double sum[kWarps];
+  float max[kWarps], bound[kWarps];
+  double lse[kMaxBeams];
+  int kind[kMaxBeams];  // 0 live, 1 finished, 2 none
+  int count;
 };
 
-// The n keys of sh.list into the K largest in order (all keys differ): each
-// key's place is the number of larger ones.
+__device__ __forceinline__ unsigned int ordered(float x) {
+  const unsigned int u = __float_as_uint(x);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(unsigned int u) {
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+__device__ __forceinline__ unsigned long long ordered(double x) {
+  const unsigned long long u = (unsigned long long)__double_as_longlong(x);
+  return (u >> 63) ? ~u : (u | (1ull << 63));
+}
+__device__ __forceinline__ double unordered(unsigned long long u) {
+  return __longlong_as_double((long long)((u >> 63) ? (u & ~(1ull << 63)) : ~u));
+}
+
+// The n keys of list into the K largest in order (all keys differ): each key's
+// place is the number of larger ones.
 __device__ void order_list(const unsigned long long* list, int n, int K, unsigned long long* out) {
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const unsigned long long k = list[i];
     int at = 0;
-    for (int j = 0; j < n && at < K; ++j) at += list[j] > k;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) at += list[j] > k;
     if (at < K) out[at] = k;
   }
 }
 
-template <typename T>
-__device__ void scan_part(SelectShared& sh, Part& out, const T* row, int v0, int v1, int K) {
+// K-th largest of the warp's 32 values (bitonic sort, descending)
+__device__ __forceinline__ float warp_kth(float v, int K) {
+  unsigned int x = ordered(v);
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const unsigned int y = __shfl_xor_sync(0xffffffffu, x, j);
+      const bool up = ((lane & k) == 0) == ((lane & j) == 0);  // this lane keeps the larger
+      x = up ? max(x, y) : min(x, y);
+    }
+  return unordered(__shfl_sync(0xffffffffu, x, K - 1));
+}
+
+// exp(x - base) for base >= x: the special-function unit's error, 2^-22, and
+// 2^-24 of the exponent
+__device__ __forceinline__ float exp_below(float x, float base) { return ex2_approx((x - base) * 1.44269504f); }
+
+template <typename T, bool ALIGNED>
+__device__ void scan_part(SelectShared& sh, const T* row, int v0, int v1, int K) {
+  constexpr int VE = 16 / sizeof(T);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  float tmax = -INFINITY;
+  Part& out = sh.mine;
+  // ---- pass 1: the largest value and the sum (a NaN or +inf makes it NaN)
+  constexpr float kLowest = -3.402823466e38f;
+  float tmax = kLowest;
   double tsum = 0.0;
-  bool nan = false;
-  int have = 0;  // keys in out so far
-  for (int blk = v0; blk < v1; blk += kBlock) {
-    float x[kPer];
-    unsigned long long best = 0;
-    float bmax = -INFINITY;
+  each_group<T, ALIGNED>(row, v0, v1, [&](const float (&x)[VE], int, int, int) {
+    float m = x[0];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int v = blk + i * kThreads + tid;
-      x[i] = v < v1 ? load_f<T>(row + v) : -INFINITY;
-      nan |= x[i] != x[i];
-      if (x[i] != x[i]) x[i] = -INFINITY;
-      bmax = fmaxf(bmax, x[i]);
+    for (int e = 1; e < VE; ++e) m = fmaxf(m, x[e]);
+    if (m > tmax) {
+      tsum *= (double)exp_below(tmax, m);
+      tmax = m;
     }
-    if (bmax > tmax) {
-      tsum *= (double)expf(tmax - bmax);
-      tmax = bmax;
-    }
-    const float base = tmax == -INFINITY ? 0.f : tmax;
+    // each term into f64: next to the row's largest term a sum in f32 would
+    // lose what tells two rows apart
+    double s0 = 0.0, s1 = 0.0;
 #pragma unroll
-    for (int i = 0; i < kPer; i += 4)
-      tsum += (double)((expf(x[i] - base) + expf(x[i + 1] - base)) + (expf(x[i + 2] - base) + expf(x[i + 3] - base)));
-    // first index of the thread's largest value
-#pragma unroll
-    for (int i = kPer - 1; i >= 0; --i) {
-      const int v = blk + i * kThreads + tid;
-      if (v < v1 && x[i] == bmax) best = make_key(x[i], v);
+    for (int e = 0; e < VE; e += 2) {
+      s0 += (double)exp_below(x[e], tmax);
+      s1 += (double)exp_below(x[e + 1], tmax);
     }
-    // ---- a bound that K keys reach: the K-th largest of the threads' largest
-    sh.best[tid] = best;
-    if (tid == 0) sh.count = 0, sh.thr = 1;
-    __syncthreads();
-    {
-      int at = 0;
-      for (int j = 0; j < kThreads; ++j) at += sh.best[j] > best;
-      if (at == K - 1 && best) sh.thr = best;
-    }
-    __syncthreads();
-    // ---- gather: at most K threads hold a key at or above it
-    unsigned long long thr = sh.thr;
-    if (have == K && out.key[K - 1] > thr) thr = out.key[K - 1];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int v = blk + i * kThreads + tid;
-      if (v < v1) {
-        const unsigned long long k = make_key(x[i], v);
-        if (k >= thr) sh.list[atomicAdd(&sh.count, 1)] = k;
-      }
-    }
-    if (tid < have) sh.list[atomicAdd(&sh.count, 1)] = out.key[tid];
-    __syncthreads();
-    const int n = sh.count;
-    order_list(sh.list, n, K, out.key);
-    have = min(n, K);
-    __syncthreads();
-  }
-  // ---- join the sums
+    tsum += s0 + s1;
+  });
+  const float kth = warp_kth(tmax == kLowest ? -INFINITY : tmax, K);
   float m = tmax;
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-  if (lane == 0) sh.max[warp] = m;
-  if (tid == 0) sh.nan = 0;
-  __syncthreads();
-  m = sh.max[0];
-#pragma unroll
-  for (int w = 1; w < kThreads / 32; ++w) m = fmaxf(m, sh.max[w]);
-  if (nan) sh.nan = 1;
-  double s = tmax == -INFINITY ? 0.0 : tsum * (double)expf(tmax - m);
+  double s = tsum * (double)exp_below(tmax, m);
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-  if (lane == 0) sh.sum[warp] = s;
+  if (lane == 0) {
+    sh.bound[warp] = kth;
+    sh.max[warp] = m;
+    sh.sum[warp] = s;
+  }
+  if (tid == 0) sh.count = 0;
   __syncthreads();
+  float bound = sh.bound[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) bound = fmaxf(bound, sh.bound[w]);
+  // ---- pass 2: what reaches the bound
+  each_group<T, ALIGNED>(row, v0, v1, [&](const float (&x)[VE], int v, int n, int step) {
+    float m = x[0];
+#pragma unroll
+    for (int e = 1; e < VE; ++e) m = fmaxf(m, x[e]);
+    if (m >= bound) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (e < n && x[e] >= bound) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kCap) sh.list[at] = make_key(x[e], v + e * step);
+        }
+    }
+  });
+  __syncthreads();
+  const int n = sh.count;
+  if (n <= kCap) {
+    order_list(sh.list, n, K, out.key);
+  } else {
+    // too many equal values: the keys one after another, each the largest
+    // below the one before
+    unsigned long long before = ~0ull;
+    for (int j = 0; j < K; ++j) {
+      unsigned long long best = 0;
+      each_group<T, ALIGNED>(row, v0, v1, [&](const float (&x)[VE], int v, int cnt, int step) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const unsigned long long k = make_key(x[e], v + e * step);
+          if (e < cnt && x[e] == x[e] && k < before && k > best) best = k;
+        }
+      });
+#pragma unroll
+      for (int k = 16; k > 0; k >>= 1) {
+        const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, k);
+        best = y > best ? y : best;
+      }
+      if (lane == 0) sh.best[warp] = best;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) best = sh.best[w] > best ? sh.best[w] : best;
+      if (tid == 0) out.key[j] = best;
+      before = best;
+      __syncthreads();
+    }
+  }
   if (tid == 0) {
+    m = sh.max[0];
+    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sh.max[w]);
     s = 0.0;
-    for (int w = 0; w < kThreads / 32; ++w) s += sh.sum[w];
-    out.sum = sh.nan ? (double)NAN : s;
+    for (int w = 0; w < kWarps; ++w) s += sh.sum[w] * (double)exp_below(sh.max[w], m);
+    out.sum = s;
     out.max = m;
-    out.n = have;
+    out.n = min(n, K);
   }
   __syncthreads();
 }
 
 // chunks: parts of a row (CTA r takes part r % chunks of rows r / chunks, + C / chunks, ...)
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_beam_select(const BeamSelectArgs a, int chunks) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  SelectShared& sh = *reinterpret_cast<SelectShared*>(smem);
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, 4) k_beam_select(const BeamSelectArgs a, int chunks) {
+  __shared__ SelectShared sh;
   uint32_t C;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
   const int rank = (int)cluster_ctarank(), b = blockIdx.x / (int)C, tid = threadIdx.x;
   const int K = a.K, lanes = (int)C / chunks;  // rows that the cluster scans at a time
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA runs
   pdl_wait();
   pdl_trigger();
-  const int chunk = rank % chunks, per = (a.V + chunks - 1) / chunks;
-  int slot = 0;
-  for (int beam = rank / chunks; beam < K; beam += lanes, ++slot) {
+  bool started = false;
+  const int chunk = rank % chunks, per = ((a.V + chunks - 1) / chunks + 7) / 8 * 8;
+  for (int beam = rank / chunks; beam < K; beam += lanes) {
     const T* row = reinterpret_cast<const T*>(a.logits) + (long long)(b * (long long)K + beam) * a.ld;
-    scan_part<T>(sh, sh.part[slot], row, chunk * per, min(a.V, (chunk + 1) * per), K);
-  }
-  cluster_sync();
-  if (rank == 0) {
-    // ---- candidates of every row: (score, beam * V + token)
-    long long* c_at = reinterpret_cast<long long*>(smem + sizeof(SelectShared));
-    double* cs = reinterpret_cast<double*>(c_at + kMaxBeams * (kMaxBeams + 1));
-    __shared__ int s_n;
-    __shared__ double s_lse[kMaxBeams];
-    __shared__ int s_kind[kMaxBeams];  // 0 live, 1 finished, 2 none
-    if (tid == 0) s_n = 0;
-    auto remote = [&](int beam, int ch) -> const Part* {
-      const uint32_t local = smem_u32(&sh.part[beam / lanes]);
-      const uint32_t addr = mapa_shared(local, (uint32_t)(beam % lanes * chunks + ch));
-      uint64_t g;
-      asm("cvta.shared::cluster.u64 %0, %1;" : "=l"(g) : "l"((uint64_t)addr));
-      return reinterpret_cast<const Part*>(g);
-    };
-    if (tid < K) {
-      float m = -INFINITY;
-      for (int ch = 0; ch < chunks; ++ch) m = fmaxf(m, remote(tid, ch)->max);
-      double s = 0.0;
-      for (int ch = 0; ch < chunks; ++ch) {
-        const Part* p = remote(tid, ch);
-        // a part of -inf alone adds nothing
-        if (p->max != -INFINITY || p->sum != p->sum) s += p->sum * (double)expf(p->max - m);
-      }
-      const float cum = a.cum[(long long)b * K + tid];
-      const bool fin = a.finished && a.finished[(long long)b * K + tid];
-      s_kind[tid] = cum != cum || cum == -INFINITY ? 2 : fin ? 1 : isfinite(s) && isfinite(m) ? 0 : 2;
-      s_lse[tid] = (double)m + log(s);
-    }
+    scan_part<T, ALIGNED>(sh, row, min(a.V, chunk * per), min(a.V, (chunk + 1) * per), K);
+    // to the first CTA's part [beam][chunk], word by word
+    if (!started) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all of them run
+    started = true;
+    const uint32_t dst = mapa_shared(smem_u32(&sh.part[beam * chunks + chunk]), 0);
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(&sh.mine);
+    if (tid < (int)(sizeof(Part) / 4))
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + 4 * tid), "r"(src[tid]) : "memory");
     __syncthreads();
-    // each row's K best of its parts' lists (one candidate a thread and step)
-    for (int i = tid; i < K * (K + 1); i += kThreads) {
-      const int beam = i / (K + 1), j = i % (K + 1);
-      const int kind = s_kind[beam];
-      double sc = -INFINITY;
-      long long at = -1;
-      if (kind == 0) {
-        // j-th of the parts' merged lists: found by its place
-        int need = j;
-        unsigned long long pick = 0;
-        if (j < K) {
-          int head[kMaxCluster];
-          for (int ch = 0; ch < chunks; ++ch) head[ch] = 0;
-          for (; need >= 0; --need) {
-            pick = 0;
-            int from = 0;
-            for (int ch = 0; ch < chunks; ++ch) {
-              const Part* p = remote(beam, ch);
-              if (head[ch] < p->n && p->key[head[ch]] > pick) pick = p->key[head[ch]], from = ch;
-            }
-            ++head[from];
-          }
-        }
-        if (pick) {
-          at = (long long)beam * a.V + key_index(pick);
-          sc = (double)a.cum[(long long)b * K + beam] + ((double)key_value(pick) - s_lse[beam]);
-        }
-      } else if (kind == 1) {
-        // the end token first, then the lowest of the others
-        const int v = j == 0 ? a.eos : (j - 1 < a.eos ? j - 1 : j);
-        if (v < a.V) {
-          at = (long long)beam * a.V + v;
-          sc = j == 0 ? (double)a.cum[(long long)b * K + beam] : -INFINITY;
-        }
-      } else if (j < a.V) {
-        at = (long long)beam * a.V + j;
-      }
-      cs[i] = sc;
-      c_at[i] = at;
-    }
-    __syncthreads();
-    const int n = K * (K + 1);
-    for (int i = tid; i < n; i += kThreads) {
-      if (c_at[i] < 0) continue;
-      int place = 0;
-      for (int j = 0; j < n && place < K; ++j)
-        place += c_at[j] >= 0 && (cs[j] > cs[i] || (cs[j] == cs[i] && c_at[j] < c_at[i]));
-      if (place < K) {
-        const int beam = (int)(c_at[i] / a.V), tok = (int)(c_at[i] - (long long)beam * a.V);
-        const long long o = (long long)b * K + place;
-        a.score[o] = (float)cs[i];
-        a.parent[o] = beam;
-        a.token[o] = tok;
-        if (a.finished_out) sh.best[place] = (tok == a.eos || s_kind[beam] == 1 || (a.finished && a.finished[(long long)b * K + beam])) ? 1 : 0;
-      }
-    }
-    __syncthreads();  // the flags read above may be the ones written here
-    if (a.finished_out && tid < K) a.finished_out[(long long)b * K + tid] = (uint8_t)sh.best[tid];
   }
-  cluster_sync();  // the parts are read until here
+  if (!started) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  cluster_sync();  // every part has arrived
+  if (rank != 0) return;
+  const float* cum = a.cum + (long long)b * K;
+  const uint8_t* fin = a.finished ? a.finished + (long long)b * K : nullptr;
+  if (tid < K) {
+    const Part* p = &sh.part[tid * chunks];
+    float m = -INFINITY;
+    for (int ch = 0; ch < chunks; ++ch) m = fmaxf(m, p[ch].max);
+    double s = 0.0;
+    for (int ch = 0; ch < chunks; ++ch) s += p[ch].sum * (double)exp_below(p[ch].max, m);
+    const float cm = cum[tid];
+    sh.kind[tid] = cm != cm || cm == -INFINITY ? 2 : fin && fin[tid] ? 1 : s > 0.0 && isfinite(s) && isfinite(m) ? 0 : 2;
+    sh.lse[tid] = (double)m + log(s);
+  }
+  __syncthreads();
+  // ---- candidates: the parts' keys; of a finished row its end token, then the
+  // lowest others; of a row that offers nothing its lowest tokens
+  const int n = K * chunks * K;
+  for (int i = tid; i < n; i += kThreads) {
+    const int j = i % K, part = i / K, beam = part / chunks, first = part % chunks == 0;
+    const int kind = sh.kind[beam];
+    double sc = -INFINITY;
+    int tok = -1;
+    if (kind == 0) {
+      if (j < sh.part[part].n) {
+        const unsigned long long k = sh.part[part].key[j];
+        tok = key_index(k);
+        sc = (double)cum[beam] + ((double)key_value(k) - sh.lse[beam]);
+      }
+    } else if (first && j < a.V) {
+      tok = kind == 2 ? j : j == 0 ? a.eos : j - 1 < a.eos ? j - 1 : j;
+      if (kind == 1 && j == 0) sc = (double)cum[beam];
+    }
+    sh.cand.score[i] = ordered(sc);
+    sh.cand.at[i] = tok < 0 ? -1 : (long long)beam * a.V + tok;
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += kThreads) {
+    const unsigned long long si = sh.cand.score[i];
+    const long long ai = sh.cand.at[i];
+    if (ai < 0) continue;
+    int place = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const unsigned long long sj = sh.cand.score[j];
+      const long long aj = sh.cand.at[j];
+      place += aj >= 0 && (sj > si || (sj == si && aj < ai));
+    }
+    if (place < K) {
+      const int beam = i / (K * chunks), tok = (int)(ai - (long long)beam * a.V);
+      const long long o = (long long)b * K + place;
+      sh.best[place] = (tok == a.eos || (fin && fin[beam])) ? 1 : 0;
+      a.parent[o] = beam;
+      a.token[o] = tok;
+      sh.part[place].sum = unordered(si);
+    }
+  }
+  __syncthreads();  // cum and finished, which these may be, have been read
+  if (tid < K) {
+    a.score[(long long)b * K + tid] = (float)sh.part[tid].sum;
+    if (a.finished_out) a.finished_out[(long long)b * K + tid] = (uint8_t)sh.best[tid];
+  }
 }
 
 // state[o][b * K + k] <- state[o][b * K + parent[b, k]], in place: a thread
@@ -334,16 +415,8 @@ cudaError_t reorder_v(const BeamReorderArgs& a, cudaStream_t st) {
   return launch_pdl(k_beam_reorder<V, 32>, grid, block, 0, st, a);
 }
 
-template <typename T>
+template <typename T, bool ALIGNED>
 cudaError_t select_t(const BeamSelectArgs& a, cudaStream_t st) {
-  auto kern = k_beam_select<T>;
-  static PerDevice once;
-  int unused = 0;
-  constexpr int smem = sizeof(SelectShared) + kMaxBeams * (kMaxBeams + 1) * 16;
-  const cudaError_t ae = per_device(once, &unused, [&](int, int&) {
-    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  });
-  if (ae != cudaSuccess) return ae;
   // CTAs of an item: a row each, or parts of a row where there are few rows
   // and the parts are not short
   int chunks = 1;
@@ -352,7 +425,6 @@ cudaError_t select_t(const BeamSelectArgs& a, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.B * C));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -362,14 +434,17 @@ cudaError_t select_t(const BeamSelectArgs& a, cudaStream_t st) {
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kern, a, chunks);
+  return cudaLaunchKernelEx(&cfg, k_beam_select<T, ALIGNED>, a, chunks);
 }
 
 }  // namespace
 
 cudaError_t beam_select_launch(const BeamSelectArgs& a, int dtype, cudaStream_t st) {
   if (a.B <= 0) return cudaSuccess;
-  return dtype == 0 ? select_t<__half>(a, st) : dtype == 1 ? select_t<__nv_bfloat16>(a, st) : select_t<float>(a, st);
+  const bool al = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.ld % (dtype == 2 ? 4 : 8) == 0;
+  if (dtype == 0) return al ? select_t<__half, true>(a, st) : select_t<__half, false>(a, st);
+  if (dtype == 1) return al ? select_t<__nv_bfloat16, true>(a, st) : select_t<__nv_bfloat16, false>(a, st);
+  return al ? select_t<float, true>(a, st) : select_t<float, false>(a, st);
 }
 
 cudaError_t beam_reorder_launch(const BeamReorderArgs& a, cudaStream_t st) {

@@ -579,6 +579,12 @@ def test_beam_select_ties(cuda, B, K, V):
     flat = logits.double().flatten(1)
     at = torch.sort(flat, dim=1, descending=True, stable=True)[1][:, :K]
     assert torch.equal(parent.long(), at // V) and torch.equal(token.long(), at % V)
+    # the same rows on 16-byte boundaries, and in 16 bits
+    for dt, pad in ((torch.float32, (-V) % 4), (torch.float16, (-V) % 8), (torch.float16, 1)):
+        wide = torch.zeros(B, K, V + pad, dtype=dt, device=cuda)
+        wide[..., :V] = logits
+        _, parent, token, _ = run_select(wide[..., :V], cum, no, V - 1)
+        assert torch.equal(parent.long(), at // V) and torch.equal(token.long(), at % V)
     # constant rows: tokens 0 .. of beam 0
     _, parent, token, _ = run_select(torch.full_like(logits, -3.5), cum, no, V - 1)
     want = torch.arange(K, device=cuda).expand(B, K)
