@@ -106,18 +106,10 @@ struct Part {
 struct SelectShared {
   Part part[kMaxBeams];  // in the cluster's first CTA: those of [row][part of it]
   Part mine;
-  union {
-    unsigned long long list[kCap];
-    struct {
-      unsigned long long score[kMaxBeams * kMaxBeams];  // ordered bits of the candidates' scores
-      long long at[kMaxBeams * kMaxBeams];              // beam * V + token, or -1
-    } cand;
-  };
+  unsigned long long list[kCap];
   unsigned long long best[kMaxBeams];
   double sum[kWarps];
   float max[kWarps], bound[kWarps];
-  double lse[kMaxBeams];
-  int kind[kMaxBeams];  // 0 live, 1 finished, 2 none
   int count;
 };
 
@@ -132,19 +124,23 @@ __device__ __forceinline__ unsigned long long ordered(double x) {
   const unsigned long long u = (unsigned long long)__double_as_longlong(x);
   return (u >> 63) ? ~u : (u | (1ull << 63));
 }
-__device__ __forceinline__ double unordered(unsigned long long u) {
-  return __longlong_as_double((long long)((u >> 63) ? (u & ~(1ull << 63)) : ~u));
-}
 
 // The n keys of list into the K largest in order (all keys differ): each key's
-// place is the number of larger ones.
+// place is the number of larger ones. Four threads count for a key where there
+// are few.
 __device__ void order_list(const unsigned long long* list, int n, int K, unsigned long long* out) {
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const unsigned long long k = list[i];
+  const int share = n <= kThreads / 4 ? 4 : 1, first = threadIdx.x % share;
+  for (int base = 0; base < n; base += kThreads / share) {
+    const int i = base + threadIdx.x / share;
+    const unsigned long long k = i < n ? list[i] : ~0ull;
     int at = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) at += list[j] > k;
-    if (at < K) out[at] = k;
+#pragma unroll 8
+    for (int j = first; j < n; j += share) at += list[j] > k;
+    if (share == 4) {
+      at += __shfl_xor_sync(0xffffffffu, at, 1);
+      at += __shfl_xor_sync(0xffffffffu, at, 2);
+    }
+    if (i < n && first == 0 && at < K) out[at] = k;
   }
 }
 
@@ -211,8 +207,8 @@ __device__ void scan_part(SelectShared& sh, const T* row, int v0, int v1, int K)
   float bound = sh.bound[0];
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) bound = fmaxf(bound, sh.bound[w]);
-  // ---- pass 2: what reaches the bound
-  each_group<T, ALIGNED>(row, v0, v1, [&](const float (&x)[VE], int v, int n, int step) {
+  // ---- pass 2: what reaches the bound (few threads hold any)
+  if (tmax >= bound || bound == -INFINITY) each_group<T, ALIGNED>(row, v0, v1, [&](const float (&x)[VE], int v, int n, int step) {
     float m = x[0];
 #pragma unroll
     for (int e = 1; e < VE; ++e) m = fmaxf(m, x[e]);
@@ -295,66 +291,68 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_select(const BeamSelectArg
   }
   if (!started) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   cluster_sync();  // every part has arrived
-  if (rank != 0) return;
-  const float* cum = a.cum + (long long)b * K;
-  const uint8_t* fin = a.finished ? a.finished + (long long)b * K : nullptr;
-  if (tid < K) {
-    const Part* p = &sh.part[tid * chunks];
-    float m = -INFINITY;
-    for (int ch = 0; ch < chunks; ++ch) m = fmaxf(m, p[ch].max);
-    double s = 0.0;
-    for (int ch = 0; ch < chunks; ++ch) s += p[ch].sum * (double)exp_below(p[ch].max, m);
-    const float cm = cum[tid];
-    sh.kind[tid] = cm != cm || cm == -INFINITY ? 2 : fin && fin[tid] ? 1 : s > 0.0 && isfinite(s) && isfinite(m) ? 0 : 2;
-    sh.lse[tid] = (double)m + log(s);
-  }
-  __syncthreads();
-  // ---- candidates: the parts' keys; of a finished row its end token, then the
-  // lowest others; of a row that offers nothing its lowest tokens
-  const int n = K * chunks * K;
-  for (int i = tid; i < n; i += kThreads) {
-    const int j = i % K, part = i / K, beam = part / chunks, first = part % chunks == 0;
-    const int kind = sh.kind[beam];
+  if (rank != 0 || tid >= 32) return;
+  // ---- the first warp takes the K best off the heads of the lists, a lane a
+  // list (K * chunks <= 32); the lowest lane among equal scores has the lowest
+  // beam and, of a row's parts, the lowest tokens
+  const int beam = tid / chunks;
+  const bool on = beam < K;
+  const Part* rows = &sh.part[on ? beam * chunks : 0];
+  float m = -INFINITY;
+  for (int ch = 0; ch < chunks; ++ch) m = fmaxf(m, rows[ch].max);
+  double s = 0.0;
+  for (int ch = 0; ch < chunks; ++ch) s += rows[ch].sum * (double)exp_below(rows[ch].max, m);
+  const float cum = on ? a.cum[(long long)b * K + beam] : -INFINITY;
+  const bool fin = on && a.finished && a.finished[(long long)b * K + beam];
+  // 0: a live row; 1: finished, its end token, then the lowest others; 2: one
+  // that offers nothing, its lowest tokens
+  const int kind = cum != cum || cum == -INFINITY ? 2 : fin ? 1 : s > 0.0 && isfinite(s) && isfinite(m) ? 0 : 2;
+  const double lse = (double)m + log(s);
+  const Part& mine = sh.part[on ? tid : 0];
+  const bool lists = on && (kind == 0 || tid % chunks == 0);
+  const int len = !lists ? 0 : kind == 0 ? mine.n : min(a.V, K);
+  int j = 0, tok = -1;
+  unsigned long long head = 0;  // ordered bits of the score; 0: the list is empty
+  auto next = [&]() {
+    head = 0;
+    if (j >= len) return;
     double sc = -INFINITY;
-    int tok = -1;
     if (kind == 0) {
-      if (j < sh.part[part].n) {
-        const unsigned long long k = sh.part[part].key[j];
-        tok = key_index(k);
-        sc = (double)cum[beam] + ((double)key_value(k) - sh.lse[beam]);
-      }
-    } else if (first && j < a.V) {
+      const unsigned long long k = mine.key[j];
+      tok = key_index(k);
+      sc = (double)cum + ((double)key_value(k) - lse);
+    } else {
       tok = kind == 2 ? j : j == 0 ? a.eos : j - 1 < a.eos ? j - 1 : j;
-      if (kind == 1 && j == 0) sc = (double)cum[beam];
+      if (kind == 1 && j == 0) sc = (double)cum;
     }
-    sh.cand.score[i] = ordered(sc);
-    sh.cand.at[i] = tok < 0 ? -1 : (long long)beam * a.V + tok;
+    head = ordered(sc);
+    ++j;
+  };
+  next();
+  float score = 0.f;
+  int parent = 0, token = 0, done = 0;  // of place tid
+  for (int place = 0; place < K; ++place) {
+    const unsigned int hi = (unsigned int)(head >> 32), top = __reduce_max_sync(0xffffffffu, hi);
+    const unsigned int lo = hi == top ? (unsigned int)head : 0u, low = __reduce_max_sync(0xffffffffu, lo);
+    const int from = __ffs(__ballot_sync(0xffffffffu, hi == top && lo == low && head != 0)) - 1;
+    const unsigned long long best = ((unsigned long long)top << 32) | low;
+    const int t = __shfl_sync(0xffffffffu, tok, from), f = __shfl_sync(0xffffffffu, (int)fin, from);
+    if (tid == place) {
+      const double sc = __longlong_as_double((long long)((best >> 63) ? (best & ~(1ull << 63)) : ~best));
+      score = (float)sc;
+      parent = from / chunks;
+      token = t;
+      done = t == a.eos || f;
+    }
+    if (tid == from) next();
   }
-  __syncthreads();
-  for (int i = tid; i < n; i += kThreads) {
-    const unsigned long long si = sh.cand.score[i];
-    const long long ai = sh.cand.at[i];
-    if (ai < 0) continue;
-    int place = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-      const unsigned long long sj = sh.cand.score[j];
-      const long long aj = sh.cand.at[j];
-      place += aj >= 0 && (sj > si || (sj == si && aj < ai));
-    }
-    if (place < K) {
-      const int beam = i / (K * chunks), tok = (int)(ai - (long long)beam * a.V);
-      const long long o = (long long)b * K + place;
-      sh.best[place] = (tok == a.eos || (fin && fin[beam])) ? 1 : 0;
-      a.parent[o] = beam;
-      a.token[o] = tok;
-      sh.part[place].sum = unordered(si);
-    }
-  }
-  __syncthreads();  // cum and finished, which these may be, have been read
+  // (cum and finished, which these may be, have been read)
   if (tid < K) {
-    a.score[(long long)b * K + tid] = (float)sh.part[tid].sum;
-    if (a.finished_out) a.finished_out[(long long)b * K + tid] = (uint8_t)sh.best[tid];
+    const long long o = (long long)b * K + tid;
+    a.score[o] = score;
+    a.parent[o] = parent;
+    a.token[o] = token;
+    if (a.finished_out) a.finished_out[o] = (uint8_t)done;
   }
 }
 
