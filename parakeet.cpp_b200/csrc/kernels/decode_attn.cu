@@ -38,6 +38,7 @@
 // 11), which the softmax's factor takes back.
 #include "common.cuh"
 #include "decode.h"
+#include "decode_common.cuh"
 #include "per_device.h"
 
 namespace pkc {
@@ -77,37 +78,6 @@ __device__ __forceinline__ uint32_t e4m3_hi(uint32_t w) {
   uint32_t r;
   asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
   return r;
-}
-
-// One item's share of a call, checked against the sizes that the host knows.
-struct Item {
-  int q0, n, len, kv0;
-  bool ok;
-};
-template <bool Q8>
-__device__ __forceinline__ Item load_item(const DecodeAttnArgs& a, int b) {
-  Item it;
-  it.q0 = a.q_off[b];
-  it.n = a.q_off[b + 1] - it.q0;
-  it.len = a.kv_len[b];
-  it.kv0 = Q8 ? 0 : a.kv_off[b];
-  it.ok = it.q0 >= 0 && it.n >= 0 && it.n <= a.max_q && it.q0 <= a.q_rows - it.n && it.len >= 0 && it.len <= a.max_kv;
-  if (Q8)
-    it.ok = it.ok && it.n <= it.len;
-  else
-    it.ok = it.ok && it.kv0 >= 0 && it.kv0 <= a.kv_rows - it.len;
-  return it;
-}
-
-// keys that row i (token i of n) sees
-template <bool Q8>
-__device__ __forceinline__ int visible(const Item& it, int i) {
-  return Q8 ? it.len - it.n + i + 1 : it.len;
-}
-
-// index of a block of rows
-__device__ __forceinline__ long long part_at(const DecodeAttnArgs& a, int row_tiles, int b, int h, int rt) {
-  return ((long long)b * a.n_kv_heads + h) * row_tiles + rt;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -675,6 +645,7 @@ __global__ void __launch_bounds__(128) k_attn_join(const DecodeAttnArgs a, int r
 #pragma unroll 4
   for (int s = warp; s < n_split; s += 4) {
     const float2 ml = *reinterpret_cast<const float2*>(p + s * PS + R * D + 2 * r);
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // a part without keys leaves its sums unwritten
     const float f = ex2_approx(ml.x - base);
     l = fmaf(ml.y, f, l);
 #pragma unroll
@@ -695,26 +666,41 @@ __global__ void __launch_bounds__(128) k_attn_join(const DecodeAttnArgs a, int r
   }
 }
 
-// How a call is cut.
+// How a call is cut. (tiles: false for what the tcgen05 kernel cannot describe,
+// which then needs no workspace either.)
+//  - Items of more than kFewRows rows: tiles of 128 rows on tcgen05
+//    (decode_attn_tc.cu), the keys in parts where there are few tiles.
 //  - Blocks of 8 rows, or of 16 where an item has more: they share one read of
 //    the keys.
 //  - Many blocks: a warp takes one alone (CTAs of one warp, no join).
 //  - Else four warps share a part, and the keys are cut into as many parts as
 //    give about six CTAs an SM (lengths differ; two run at a time), of at
 //    least 128 keys.
+constexpr int kFewRows = 32;
 struct Plan {
-  int rows, row_tiles, warps, n_split;
+  int rows, row_tiles, warps, n_split;  // warps 0: the tcgen05 kernel
   long long blocks;
 };
-Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads) {
+Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, bool tiles = true) {
   Plan p;
   const long long rows = (long long)max_q * (n_heads / n_kv_heads);
+  if (rows > kFewRows && tiles) {
+    p.rows = kTileRows;
+    p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
+    p.blocks = (long long)n_items * n_kv_heads * p.row_tiles;
+    p.warps = 0;
+    // two CTAs run on an SM: parts of at least 512 keys until all have one
+    const long long want = (2LL * kSms) / (p.blocks > 0 ? p.blocks : 1), most = (max_kv + 511) / 512;
+    const long long n = want < most ? want : most;
+    p.n_split = n < 1 ? 1 : n > 64 ? 64 : (int)n;
+    return p;
+  }
   p.rows = rows <= 8 ? 8 : 16;
   p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
   p.blocks = (long long)n_items * n_kv_heads * p.row_tiles;
   p.warps = 1;
   p.n_split = 1;
-  if (p.blocks < 8LL * kSms) {
+  if (p.blocks < 8LL * kSms && tiles) {
     p.warps = 4;
     const long long want = (6LL * kSms + p.blocks - 1) / (p.blocks > 0 ? p.blocks : 1);
     const long long most = (max_kv + 127) / 128;
@@ -742,8 +728,14 @@ cudaError_t launch_w(const DecodeAttnArgs& a, const Plan& p, cudaStream_t st) {
 
 template <typename H, bool Q8, int D, int WT>
 cudaError_t launch_rows(const DecodeAttnArgs& a, cudaStream_t st) {
-  const Plan p = plan_rows(a.n_items, a.max_q, a.max_kv, a.n_heads, a.n_kv_heads);
-  if (p.blocks * p.n_split * 16 > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const Plan p = plan_rows(a.n_items, a.max_q, a.max_kv, a.n_heads, a.n_kv_heads, attn_tiles_fit(a));
+  if (p.blocks * p.n_split * p.rows > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (p.warps == 0) {
+    const cudaError_t e = attn_tiles_launch(a, is_bf16<H>::value, p.row_tiles, p.n_split, st);
+    if (e != cudaSuccess || p.n_split == 1) return e;
+    return launch_pdl(k_attn_join<H, Q8, D, kTileRows>, dim3((unsigned)(p.blocks * kTileRows)), dim3(128), 0, st, a,
+                      p.row_tiles, p.n_split);
+  }
   if (p.rows == 8)
     return p.warps == 1 ? launch_w<H, Q8, D, WT, 1, 1>(a, p, st) : launch_w<H, Q8, D, WT, 4, 1>(a, p, st);
   return p.warps == 1 ? launch_w<H, Q8, D, WT, 1, 2>(a, p, st) : launch_w<H, Q8, D, WT, 4, 2>(a, p, st);

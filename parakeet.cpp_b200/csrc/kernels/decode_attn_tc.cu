@@ -1,0 +1,653 @@
+// Attention of many query rows over keys and values of another length on the
+// 5th-generation tensor cores: rescoring, prompts, chunks of a prompt. The
+// operators and their masks are those of decode_attn.cu.
+//
+// One CTA takes 128 query rows (tokens x heads of one shared key head: one
+// TMEM lane each) of one item and one part of its keys, in tiles of 64 keys:
+//   S = Q K^T  (tcgen05.mma, f32 in tensor memory), p = exp2(c S - m),
+//   O += P V   (P in 16 bits in tensor memory, over the S that it came from).
+// Two CTAs share an SM (half of the tensor memory each): while one's softmax
+// runs, the other's products do. A row is a thread, so its maximum and sum
+// need no exchange; the maximum that the exponentials use moves only when it
+// is exceeded by more than 2^8, and only then is O rescaled.
+//
+// Tensor memory (256 columns x 128 lanes): S of even and odd tiles at 0 and 64
+// (the first 32 columns of each become that tile's P), O at 128.
+// Shared memory: Q (written by the softmax warps, in the 128-byte swizzle that
+// the products read), a ring of four 64-row tiles K0 K1 V0 K2 V1 ... in the
+// order of their use.
+//
+// 16-bit keys and values come by TMA. Rows behind an item's last key belong to
+// others: their scores are masked, and their values, which a zero probability
+// would not silence if they are not numbers, are zeroed in the last tile.
+//
+// The 8-bit cache's codes are turned into f16 by two warps that write the same
+// ring: exactly, with the value scale taken in as a power of two relative to a
+// reference 2^ref in which O is kept. f16 holds e4m3 codes times 2^-15 .. 2^7
+// exactly, so ref stands while the pages stay in that range of it; else it
+// moves to the tile's largest scale and O is multiplied. A tile of several
+// small pages that are further apart than that takes them one after another,
+// each under its own reference (16 keys of one product step lie in one page).
+#include "common.cuh"
+#include "decode.h"
+#include "decode_common.cuh"
+#include "gemm.h"
+#include "per_device.h"
+
+namespace pkc {
+
+namespace {
+
+constexpr int QM = kTileRows;
+constexpr int KN = 64;
+constexpr int RING = 4;
+constexpr int SOFT_WARPS = 4;
+constexpr int CVT_WARPS = 2;
+constexpr float kRescaleLog2 = 8.0f;
+constexpr uint32_t TM_O = 128, TM_COLS = 256;
+
+enum : int {
+  B_QREADY = 0, B_RFULL = 1, B_REMPTY = B_RFULL + RING, B_SFULL = B_REMPTY + RING, B_PFULL = B_SFULL + 2,
+  B_PVDONE = B_PFULL + 2, B_INFO = B_PVDONE + 2, B_FINAL = B_INFO + RING, N_BARS = B_FINAL + 1
+};
+
+// What the converting warps tell the softmax about a tile.
+struct TileInfo {
+  float ks[4];    // key scale of each 16 keys; -1: a page that is none
+  float grow[4];  // O is multiplied by this before part j of the tile is added
+  float ref;      // exponent that O is kept under, behind the tile
+  int parts;      // 1, or the tile's pages
+};
+
+template <int D>
+struct TilesLayout {
+  static constexpr int KB = D / 64;
+  static constexpr int Q_BYTES = QM * D * 2;
+  static constexpr int T_BYTES = KN * D * 2;
+  static constexpr int OFF_RING = Q_BYTES;
+  static constexpr int OFF_FACTOR = OFF_RING + RING * T_BYTES;  // [QM] softmax factors
+  static constexpr int OFF_INFO = OFF_FACTOR + QM * 4;          // [RING] TileInfo
+  static constexpr int OFF_BAR = OFF_INFO + RING * 64;
+  static constexpr int OFF_SLOT = OFF_BAR + N_BARS * 8;
+  static constexpr int SMEM = OFF_SLOT + 16 + 1024;  // + alignment slack
+};
+static_assert(sizeof(TileInfo) <= 64, "the layout gives it 64 bytes");
+
+// place of a tile in the ring's order K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1)
+__device__ __forceinline__ int at_k(int t) { return t < 2 ? t : 2 * t - 1; }
+__device__ __forceinline__ int at_v(int t, int n) { return t < n - 2 ? 2 * t + 2 : t == n - 1 ? 2 * n - 1 : 2 * n - 2; }
+
+__device__ __forceinline__ float pow2i(int e) {
+  e = e < -126 ? -126 : e > 127 ? 127 : e;
+  return __int_as_float((e + 127) << 23);
+}
+
+template <typename H, bool Q8, int D>
+__global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 2)
+    k_attn_tiles(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const DecodeAttnArgs a,
+                 int row_tiles, int n_split) {
+  using M = typename std::conditional<Q8, __half, H>::type;
+  using L = TilesLayout<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::OFF_BAR);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::OFF_SLOT);
+  float* s_factor = reinterpret_cast<float*>(sm + L::OFF_FACTOR);
+  const uint32_t sbase = smem_u32(sm);
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  auto info = [&](int t) { return reinterpret_cast<TileInfo*>(sm + L::OFF_INFO + (t % RING) * 64); };
+
+  const int G = a.n_heads / a.n_kv_heads;
+  const int split = blockIdx.x % n_split;
+  int rest = blockIdx.x / n_split;
+  const int rt = rest % row_tiles;
+  rest /= row_tiles;
+  const int h = rest % a.n_kv_heads, b = rest / a.n_kv_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
+  const Item it = load_item<Q8>(a, b);
+  if (!it.ok) {
+    if (threadIdx.x == 0) report_error(a.err, DEV_ERR_BAD_SHAPE);
+    return;
+  }
+  const int rows = it.n * G, row0 = rt * QM;
+  if (row0 >= rows) return;
+  const int valid = min(QM, rows - row0);
+  const int vmax = max(0, visible<Q8>(it, (row0 + valid - 1) / G));  // keys that some row sees
+  const int vmin = Q8 ? visible<Q8>(it, row0 / G) : vmax;            // keys that every row sees
+  const int n_all = (vmax + KN - 1) / KN, per = (n_all + n_split - 1) / n_split;
+  const int t0 = split * per;
+  const int nT = max(0, min(n_all, t0 + per) - t0);  // this CTA's tiles: t0, t0 + 1, ...
+
+  if (threadIdx.x == 0) {
+    if constexpr (!Q8) {
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+    }
+    for (int i = 0; i < N_BARS; ++i) {
+      const bool soft = i == B_QREADY || i == B_PFULL || i == B_PFULL + 1;
+      const bool full = i >= B_RFULL && i < B_RFULL + RING;
+      mbar_init(bar(i), soft ? SOFT_WARPS : full && Q8 ? CVT_WARPS : 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(tmem_slot), TM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto wwait = [&](int i, uint32_t parity) -> bool {
+    return __all_sync(0xffffffffu, mbar_wait(bar(i), parity, a.err, DEV_ERR_TIMEOUT_ATTN)) != 0;
+  };
+  // pages: tokens of a page, pages in a tile, keys of one in it
+  const int page = Q8 ? a.cache.page : KN, np = Q8 && page < KN ? KN / page : 1;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (nT > 0) {
+      const uint32_t leader = elect_one();
+      constexpr int fmt = is_bf16<M>::value ? 1 : 0;
+      constexpr uint32_t id_s = idesc_f16(QM, KN, fmt);
+      constexpr uint32_t id_pv = idesc_f16(QM, D, fmt) | (1u << 16);  // B (V) MN-major
+      const uint64_t dq = smem_desc_sw128(sbase);
+      auto ring_wait = [&](int n) -> bool {
+        if (!wwait(B_RFULL + n % RING, (uint32_t)(n / RING) & 1u)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto ring_addr = [&](int n) { return sbase + L::OFF_RING + (n % RING) * L::T_BYTES; };
+      auto s_mma = [&](int t) -> bool {
+        const int n = at_k(t);
+        if (!ring_wait(n)) return false;
+        const uint64_t dk = smem_desc_sw128(ring_addr(n));
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_f16_if(leader, tmem + 64u * (uint32_t)(t & 1), dq + (uint64_t)(((kk >> 2) * QM * 128 + (kk & 3) * 32) >> 4),
+                      dk + (uint64_t)(((kk >> 2) * KN * 128 + (kk & 3) * 32) >> 4), id_s, kk > 0 ? 1u : 0u);
+        umma_commit_if(leader, bar(B_REMPTY + n % RING));
+        umma_commit_if(leader, bar(B_SFULL + (t & 1)));
+        return true;
+      };
+      bool ok = wwait(B_QREADY, 0);
+      tc_fence_after();
+      ok = ok && s_mma(0) && (nT < 2 || s_mma(1));
+      uint32_t pf = 0;  // completed phases of the two PFULL barriers, as parities
+      for (int t = 0; t < nT && ok; ++t) {
+        const int n = at_v(t, nT), buf = t & 1;
+        if (!(ok = ring_wait(n))) break;
+        if constexpr (!Q8) {
+          const int left = vmax - (t0 + t) * KN;
+          if (left < KN) {
+            uint8_t* vt = sm + L::OFF_RING + (n % RING) * L::T_BYTES;
+            for (int i = lane; i < (KN - left) * 8 * L::KB; i += 32) {
+              const int kb = i / ((KN - left) * 8), j = i % ((KN - left) * 8);
+              *reinterpret_cast<uint4*>(vt + kb * KN * 128 + left * 128 + j * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        const uint64_t dv = smem_desc_sw128_mn(ring_addr(n), KN * 128, 1024);
+        const uint32_t pa = tmem + 64u * (uint32_t)buf;
+        const int parts = Q8 ? info(t)->parts : 1, steps = KN / 16 / parts;
+        for (int j = 0; j < parts && ok; ++j) {
+          ok = wwait(B_PFULL + buf, (pf >> buf) & 1u);
+          pf ^= 1u << buf;
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < KN / 16; ++kk)
+            if (kk / steps == j)
+              umma_f16_ts_if(leader, tmem + TM_O, pa + 8u * kk, dv + (uint64_t)((kk * 16 * 128) >> 4), id_pv,
+                             (t > 0 || kk > 0) ? 1u : 0u);
+          if (j == parts - 1) umma_commit_if(leader, bar(B_REMPTY + n % RING));
+          umma_commit_if(leader, bar(B_PVDONE + buf));
+        }
+        if (ok && t + 2 < nT) ok = s_mma(t + 2);
+      }
+      // every issued product has completed before the tensor memory goes
+      umma_commit_if(leader, bar(B_FINAL));
+      wwait(B_FINAL, 0);
+    }
+  } else if (warp <= SOFT_WARPS) {
+    // ---------------------------------------------------------------- softmax warps
+    const int q = warp & 3;  // TMEM lane quarter
+    const int i = 32 * q + lane;
+    const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16);
+    // ---- this warp's 32 rows of Q, D / 8 lanes a row
+    constexpr int CH = D / 8, RP = 32 / CH;
+#pragma unroll 4
+    for (int j = 0; j < 32 / RP; ++j) {
+      const int r = 32 * q + j * RP + lane / CH, ch = lane % CH;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (r < valid) {
+        const int rr = row0 + r;
+        w = *reinterpret_cast<const uint4*>(reinterpret_cast<const H*>(a.q) + (long long)(it.q0 + rr / G) * a.ldq +
+                                            (h * G + rr % G) * D + ch * 8);
+      }
+      if (a.scale_log2 < 0.f) {  // the factor stays positive: the largest product has the largest score
+        w.x ^= 0x80008000u;
+        w.y ^= 0x80008000u;
+        w.z ^= 0x80008000u;
+        w.w ^= 0x80008000u;
+      }
+      float factor = fabsf(a.scale_log2);
+      if constexpr (Q8 && is_bf16<H>::value) {
+        // to f16 with a power of two for the row (see decode_attn.cu)
+        const H* x = reinterpret_cast<const H*>(&w);
+        float m = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(from_h(x[k])));
+#pragma unroll
+        for (int k = CH / 2; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+        const int e = ((__float_as_int(m) >> 23) & 255) - 127;
+        const float f = m > 0.f && e < 127 && e > -126 ? __int_as_float((127 - e) << 23) : 1.f;
+        factor /= f;
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = pack2<__half>(from_h(x[2 * k]) * f, from_h(x[2 * k + 1]) * f);
+        w = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      if (ch == 0) s_factor[r] = factor;
+      *reinterpret_cast<uint4*>(sm + (ch >> 3) * QM * 128 + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = w;
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(B_QREADY));
+
+    const float rs = s_factor[i];
+    const int vis = i < valid ? visible<Q8>(it, (row0 + i) / G) : 0;
+    float m_used = -INFINITY, lsum = 0.f, ref = 0.f;
+    bool ok = true;
+    uint32_t pvw = 0;        // PVDONE phases: parity to wait for next, per buffer
+    int pv_buf = -1;         // buffer of the last part handed to the MMA warp
+    uint32_t pv_par = 0;
+    // O of the parts so far is complete
+    auto o_settled = [&]() -> bool {
+      if (pv_buf < 0) return true;
+      if (!wwait(B_PVDONE + pv_buf, pv_par)) return false;
+      tc_fence_after();
+      return true;
+    };
+    auto scale_o = [&](float f) {
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(trow + TM_O + 32u * c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+        tmem_st32(trow + TM_O + 32u * c, o);
+      }
+      tmem_st_wait();
+    };
+    for (int t = 0; t < nT && ok; ++t) {
+      const int buf = t & 1, k0 = (t0 + t) * KN;
+      if (!(ok = wwait(B_SFULL + buf, (uint32_t)(t >> 1) & 1u))) break;
+      tc_fence_after();
+      TileInfo ti{};
+      if constexpr (Q8) {
+        if (!(ok = wwait(B_INFO + t % RING, (uint32_t)(t / RING) & 1u))) break;
+        ti = *info(t);
+      }
+      float x[KN];
+      {
+        uint32_t s0[32], s1[32];
+        tmem_ld32(trow + 64u * buf, s0);
+        tmem_ld32(trow + 64u * buf + 32u, s1);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          x[j] = __uint_as_float(s0[j]);
+          x[32 + j] = __uint_as_float(s1[j]);
+        }
+      }
+      float c = rs;
+      if constexpr (Q8) {
+        if (np == 1) {
+          c *= ti.ks[0];
+        } else {
+#pragma unroll
+          for (int j = 0; j < KN; ++j) x[j] *= ti.ks[j >> 4];
+        }
+      }
+      if (k0 + KN > vmin) {
+#pragma unroll
+        for (int j = 0; j < KN; ++j)
+          if (k0 + j >= vis) x[j] = -INFINITY;
+      }
+      if constexpr (Q8) {
+        if (fminf(fminf(ti.ks[0], ti.ks[1]), fminf(ti.ks[2], ti.ks[3])) < 0.f) {  // pages that are none are not seen
+#pragma unroll
+          for (int j = 0; j < KN; ++j)
+            if (ti.ks[j >> 4] < 0.f) x[j] = -INFINITY;
+          c = rs * fabsf(np == 1 ? ti.ks[0] : 1.f);
+        }
+      }
+      float mx[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        mx[k] = x[k];
+#pragma unroll
+        for (int j = 1; j < KN / 8; ++j) mx[k] = fmaxf(mx[k], x[8 * j + k]);
+      }
+      const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                             fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * c;
+      float alpha = 1.f;
+      if (mt > m_used + kRescaleLog2) {
+        alpha = ex2_approx(m_used - mt);
+        m_used = mt;
+        lsum *= alpha;
+      }
+      const float mu = m_used == -INFINITY ? 0.f : m_used;
+      uint32_t pk[KN / 2];
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KN / 2; ++j) {
+        // (a masked score under a factor of zero is not a number: zero then)
+        float p0 = ex2_approx(fmaf(x[2 * j], c, -mu)), p1 = ex2_approx(fmaf(x[2 * j + 1], c, -mu));
+        if (c == 0.f) {
+          p0 = x[2 * j] == -INFINITY ? 0.f : p0;
+          p1 = x[2 * j + 1] == -INFINITY ? 0.f : p1;
+        }
+        sum[j & 3] += p0 + p1;
+        pk[j] = pack2<M>(p0, p1);
+      }
+      lsum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st32(trow + 64u * buf, pk);
+      // ---- O: the row's maximum moved, or the reference of the values did
+      const int parts = Q8 ? ti.parts : 1;
+#pragma unroll 1
+      for (int j = 0; j < parts && ok; ++j) {
+        const float f = (j == 0 ? alpha : 1.f) * (Q8 ? ti.grow[j] : 1.f);
+        const bool scale = pv_buf >= 0 && __any_sync(0xffffffffu, f != 1.f);
+        // (a part that is not the tile's first also waits because its arrival
+        // below must not count for the part before)
+        if ((scale || j > 0) && !(ok = o_settled())) break;
+        if (scale) scale_o(f);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_PFULL + buf));
+        pv_buf = buf;
+        pv_par = (pvw >> buf) & 1u;
+        pvw ^= 1u << buf;
+      }
+      if constexpr (Q8) ref = ti.ref;
+    }
+    if (ok) ok = o_settled();
+    // ---- O / l, through this warp's rows of the Q tile (every product that
+    // reads Q is done), stored as whole rows; or the part's sums
+    if (ok) {
+      const float back = Q8 && nT > 0 ? pow2i((int)ref) : 1.f;
+      if (n_split == 1) {
+        const float inv = lsum == 0.f ? 0.f : back / lsum;  // no key seen: zeros
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (nT > 0) {
+            tmem_ld32(trow + TM_O + 32u * c, o);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = lsum == 0.f ? 0u : pack2<H>(__uint_as_float(o[8 * k + 2 * e]) * inv, __uint_as_float(o[8 * k + 2 * e + 1]) * inv);
+            *reinterpret_cast<uint4*>(sm + i * (D * 2) + (((4 * c + k) ^ (i & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        __syncwarp();
+#pragma unroll 4
+        for (int j = 0; j < 32 / RP; ++j) {
+          const int r = 32 * q + j * RP + lane / CH, ch = lane % CH, rr = row0 + r;
+          const uint4 v = *reinterpret_cast<const uint4*>(sm + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+          if (r < valid)
+            *reinterpret_cast<uint4*>(reinterpret_cast<H*>(a.out) + (long long)(it.q0 + rr / G) * a.ldo +
+                                      (h * G + rr % G) * D + ch * 8) = v;
+        }
+      } else {
+        float* po = a.ws + (part_at(a, row_tiles, b, h, rt) * n_split + split) * (QM * (D + 2));
+#pragma unroll 1
+        for (int c = 0; c < D / 32 && nT > 0; ++c) {
+          uint32_t o[32];
+          tmem_ld32(trow + TM_O + 32u * c, o);
+          tmem_ld_wait();
+          if (i < valid) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(po + i * D + 32 * c + e) =
+                  make_float4(__uint_as_float(o[e]) * back, __uint_as_float(o[e + 1]) * back,
+                              __uint_as_float(o[e + 2]) * back, __uint_as_float(o[e + 3]) * back);
+          }
+        }
+        if (i < valid) *reinterpret_cast<float2*>(po + QM * D + 2 * i) = make_float2(m_used, lsum);
+      }
+    }
+  } else if constexpr (!Q8) {
+    // ------------------------------------------------------------------ TMA producer
+    if (nT > 0) {
+      const uint32_t leader = elect_one();
+      const int n_loads = 2 * nT;
+      int n = 0, k = 0, v = 0;
+      for (; n < n_loads; ++n) {
+        const int s = n % RING;
+        if (!wwait(B_REMPTY + s, ((uint32_t)(n / RING) & 1u) ^ 1u)) break;
+        const bool is_k = k < nT && n == at_k(k);
+        const int t = is_k ? k++ : v++;
+        const CUtensorMap* map = is_k ? &tm_k : &tm_v;
+        mbar_arrive_expect_tx_if(leader, bar(B_RFULL + s), L::T_BYTES);
+#pragma unroll
+        for (int kb = 0; kb < L::KB; ++kb)
+          tma_load_2d_if(leader, sbase + L::OFF_RING + s * L::T_BYTES + kb * KN * 128, map, bar(B_RFULL + s),
+                         h * D + kb * 64, it.kv0 + (t0 + t) * KN);
+      }
+      if (n < n_loads) {
+        // a consumer gave up: every copy in flight lands before the CTA exits
+        for (int m = n - RING; m < n; ++m)
+          if (m >= 0) mbar_wait(bar(B_RFULL + m % RING), (uint32_t)(m / RING) & 1u, nullptr, 0);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ 8-bit converters
+    // Each of the two warps takes 32 of a tile's 64 rows, and both keep the
+    // same account of pages and scales (lane j < np: the tile's page j).
+    if constexpr (Q8) {
+      const Kv8& cc = a.cache;
+      const int w = warp - 1 - SOFT_WARPS;
+      constexpr int LR = D / 16, RI = 32 / LR, IT = 32 / RI;  // lanes a row, rows an iteration, iterations
+      const int r_in = lane / LR, ch = lane % LR;
+      auto page_id = [&](int t) -> int {
+        const int key = (t0 + t) * KN + lane * page;
+        return lane < np && t < nT && key < vmax ? cc.table[(long long)b * cc.table_ld + key / page] : -1;
+      };
+      int id_ahead = page_id(0), id_cur = -1, id_prev = -1;
+      float ks_ahead = 1.f, vs_ahead = 1.f;  // scales of the tile whose keys were asked for last
+      int k_asked = 0, v_asked = 0;
+      uint4 ahead[IT];
+      // ask for the codes of the next tile in the ring's order
+      auto ask = [&](int n) {
+        if (n >= 2 * nT) return;
+        const bool is_k = k_asked < nT && n == at_k(k_asked);
+        const int t = is_k ? k_asked++ : v_asked++;
+        if (is_k) {
+          id_prev = id_cur;
+          id_cur = id_ahead;
+          id_ahead = page_id(t + 1);
+          const bool on = id_cur >= 0 && id_cur < cc.n_pages;
+          ks_ahead = on ? cc.k_scale[(long long)id_cur * cc.n_kv_heads + h] : -1.f;
+          vs_ahead = on ? cc.v_scale[(long long)id_cur * cc.n_kv_heads + h] : 1.f;
+        }
+        const int ids = is_k || t == k_asked - 1 ? id_cur : id_prev;
+        const uint8_t* pool = is_k ? cc.k : cc.v;
+#pragma unroll
+        for (int j = 0; j < IT; ++j) {
+          const int r = 32 * w + j * RI + r_in, key = (t0 + t) * KN + r;
+          const int id = __shfl_sync(0xffffffffu, ids, np == 1 ? 0 : r / page);
+          ahead[j] = make_uint4(0, 0, 0, 0);
+          if (key < vmax && id >= 0 && id < cc.n_pages)
+            ahead[j] = *reinterpret_cast<const uint4*>(
+                pool + (((long long)id * cc.n_kv_heads + h) * page + key % page) * D + ch * 16);
+        }
+      };
+      int ref = 0, dv_cur = 0, dv_prev = 0, k_done = 0, v_done = 0;  // dv: lane j's page, exponent of its values' factor
+      ask(0);
+      bool ok = true;
+      for (int n = 0; n < 2 * nT && ok; ++n) {
+        uint4 codes[IT];
+#pragma unroll
+        for (int j = 0; j < IT; ++j) codes[j] = ahead[j];
+        const float ks = ks_ahead, vs = vs_ahead;
+        const int id_here = id_cur;
+        ask(n + 1);
+        const bool is_k = k_done < nT && n == at_k(k_done);
+        const int t = is_k ? k_done++ : v_done++;
+        const int s = n % RING;
+        if (!(ok = wwait(B_REMPTY + s, ((uint32_t)(n / RING) & 1u) ^ 1u))) break;
+        int dvs = 0;
+        if (is_k) {
+          // ---- the tile's scales
+          const bool in = lane < np && (t0 + t) * KN + lane * page < vmax;
+          const bool none = in && (id_here < 0 || id_here >= cc.n_pages);
+          if (none) report_error(a.err, DEV_ERR_BAD_SHAPE);
+          const int ev = ((__float_as_int(vs) >> 23) & 255) - 127;
+          const bool counts = in && !none;
+          const int mx = __reduce_max_sync(0xffffffffu, counts ? ev : -1000);
+          const int mn = __reduce_min_sync(0xffffffffu, counts ? ev : 1000);
+          float grow = 1.f;  // of part j in lane j
+          int parts = 1;
+          dv_prev = dv_cur;
+          if (mx == -1000) {  // no page: no values
+            dv_cur = 0;
+          } else if (t > 0 && mx - ref <= 7 && mn - ref >= -15) {
+            dv_cur = counts ? ev - ref : 0;  // (0: no values there)
+          } else if (mx - mn <= 15) {
+            grow = t > 0 ? pow2i(ref - mx) : 1.f;
+            ref = mx;
+            dv_cur = counts ? ev - ref : 0;
+          } else {
+            parts = np;
+            // each counting page under its own reference; from which one O comes
+            // to it: the last counting page before, or the tile before
+            const uint32_t have = __ballot_sync(0xffffffffu, counts);
+            const uint32_t before = have & ((1u << lane) - 1u);
+            const int last = 31 - __clz(have);
+            const int from = __shfl_sync(0xffffffffu, ev, before ? 31 - __clz(before) : 0);
+            grow = !counts ? 1.f : before ? pow2i(from - ev) : t > 0 ? pow2i(ref - ev) : 1.f;
+            ref = __shfl_sync(0xffffffffu, ev, last);
+            dv_cur = 0;
+          }
+          if (w == 0) {
+            const int j = lane < 4 ? (np == 1 ? 0 : lane * 16 / page) : 0;
+            const float ks_j = __shfl_sync(0xffffffffu, ks, j);
+            const bool in_j = __shfl_sync(0xffffffffu, (int)in, j);
+            TileInfo* ti = info(t);
+            if (lane < 4) {
+              ti->ks[lane] = in_j ? ks_j : 1.f;  // (keys behind the last are masked)
+              ti->grow[lane] = grow;
+            }
+            if (lane == 0) {
+              ti->ref = (float)ref;
+              ti->parts = parts;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(B_INFO + t % RING));
+          }
+        } else {
+          dvs = t == k_done - 1 ? dv_cur : dv_prev;
+        }
+        uint8_t* tile = sm + L::OFF_RING + s * L::T_BYTES;
+#pragma unroll
+        for (int j = 0; j < IT; ++j) {
+          const int r = 32 * w + j * RI + r_in;
+          const uint32_t cw[4] = {codes[j].x, codes[j].y, codes[j].z, codes[j].w};
+          uint32_t f[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+                "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+                : "=r"(f[2 * e]), "=r"(f[2 * e + 1])
+                : "r"(cw[e]));
+          }
+          if (!is_k) {
+            const int dv = __shfl_sync(0xffffffffu, dvs, np == 1 ? 0 : r / page);
+            if (__any_sync(0xffffffffu, dv != 0)) {
+              const __half2 m = __float2half2_rn(pow2i(dv < -24 ? -24 : dv));
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                __half2 y = __hmul2(*reinterpret_cast<__half2*>(&f[e]), m);
+                f[e] = *reinterpret_cast<uint32_t*>(&y);
+              }
+            }
+          }
+          // 16-byte chunks 2 ch and 2 ch + 1 of the row (the other one first
+          // in the second half of the row: fewer bank conflicts)
+          uint8_t* row = tile + (ch >> 2) * KN * 128 + r * 128;
+          const int c0 = (2 * ch) & 7, flip = (ch >> 2) & 1;
+          const uint4 lo = make_uint4(f[0], f[1], f[2], f[3]), hi = make_uint4(f[4], f[5], f[6], f[7]);
+          *reinterpret_cast<uint4*>(row + (((c0 + flip) ^ (r & 7)) << 4)) = flip ? hi : lo;
+          *reinterpret_cast<uint4*>(row + (((c0 + 1 - flip) ^ (r & 7)) << 4)) = flip ? lo : hi;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_RFULL + s));
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, TM_COLS);
+}
+
+template <typename H, bool Q8, int D>
+cudaError_t launch_tiles(const DecodeAttnArgs& a, int row_tiles, int n_split, cudaStream_t st) {
+  auto kern = k_attn_tiles<H, Q8, D>;
+  constexpr int smem = TilesLayout<D>::SMEM;
+  static PerDevice once;
+  int unused = 0;
+  const cudaError_t e = per_device(once, &unused, [&](int, int&) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  });
+  if (e != cudaSuccess) return e;
+  CUtensorMap tk{}, tv{};
+  if constexpr (!Q8) {
+    const int cols = a.n_kv_heads * D;
+    const bool bf = is_bf16<H>::value;
+    if (!make_tmap_kmajor(&tk, a.k, a.kv_rows, cols, (int)a.ldk, KN, bf) ||
+        !make_tmap_kmajor(&tv, a.v, a.kv_rows, cols, (int)a.ldv, KN, bf))
+      return cudaErrorInvalidValue;
+  }
+  const long long grid = (long long)a.n_items * a.n_kv_heads * row_tiles * n_split;
+  if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
+  return launch_pdl(kern, dim3((unsigned)grid), dim3(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1))), smem, st, tk, tv, a,
+                    row_tiles, n_split);
+}
+
+template <typename H>
+cudaError_t launch_tiles_h(const DecodeAttnArgs& a, int row_tiles, int n_split, cudaStream_t st) {
+  if (a.cache.k)
+    return a.head_dim == 128 ? launch_tiles<H, true, 128>(a, row_tiles, n_split, st)
+                             : launch_tiles<H, true, 64>(a, row_tiles, n_split, st);
+  return a.head_dim == 128 ? launch_tiles<H, false, 128>(a, row_tiles, n_split, st)
+                           : launch_tiles<H, false, 64>(a, row_tiles, n_split, st);
+}
+
+}  // namespace
+
+// A tensor map needs rows, and its stride as an int.
+bool attn_tiles_fit(const DecodeAttnArgs& a) {
+  return a.cache.k || (a.kv_rows > 0 && a.ldk <= 0x7fffffffLL && a.ldv <= 0x7fffffffLL);
+}
+
+cudaError_t attn_tiles_launch(const DecodeAttnArgs& a, bool bf16, int row_tiles, int n_split, cudaStream_t st) {
+  return bf16 ? launch_tiles_h<__nv_bfloat16>(a, row_tiles, n_split, st)
+              : launch_tiles_h<__half>(a, row_tiles, n_split, st);
+}
+
+}  // namespace pkc
