@@ -44,6 +44,7 @@ constexpr int RING = 4;
 constexpr int SOFT_WARPS = 4;
 constexpr int CVT_WARPS = 2;
 constexpr float kRescaleLog2 = 8.0f;
+constexpr float kTiny = 1e-38f;  // the least softmax factor: a masked score (-inf) times zero is not a number
 constexpr uint32_t TM_O = 128, TM_COLS = 256;
 
 enum : int {
@@ -220,15 +221,24 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
     const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16);
     // ---- this warp's 32 rows of Q, D / 8 lanes a row
     constexpr int CH = D / 8, RP = 32 / CH;
-#pragma unroll 4
+    const int ch = lane % CH;
+    // (all loads before the first store, which they might alias for all that
+    // the compiler knows)
+    uint4 qw[32 / RP];
+#pragma unroll
     for (int j = 0; j < 32 / RP; ++j) {
-      const int r = 32 * q + j * RP + lane / CH, ch = lane % CH;
-      uint4 w = make_uint4(0, 0, 0, 0);
+      const int r = 32 * q + j * RP + lane / CH;
+      qw[j] = make_uint4(0, 0, 0, 0);
       if (r < valid) {
         const int rr = row0 + r;
-        w = *reinterpret_cast<const uint4*>(reinterpret_cast<const H*>(a.q) + (long long)(it.q0 + rr / G) * a.ldq +
-                                            (h * G + rr % G) * D + ch * 8);
+        qw[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const H*>(a.q) + (long long)(it.q0 + rr / G) * a.ldq +
+                                                (h * G + rr % G) * D + ch * 8);
       }
+    }
+#pragma unroll
+    for (int j = 0; j < 32 / RP; ++j) {
+      const int r = 32 * q + j * RP + lane / CH;
+      uint4 w = qw[j];
       if (a.scale_log2 < 0.f) {  // the factor stays positive: the largest product has the largest score
         w.x ^= 0x80008000u;
         w.y ^= 0x80008000u;
@@ -259,7 +269,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(B_QREADY));
 
-    const float rs = s_factor[i];
+    const float rs = fmaxf(s_factor[i], kTiny);
     const int vis = i < valid ? visible<Q8>(it, (row0 + i) / G) : 0;
     float m_used = -INFINITY, lsum = 0.f, ref = 0.f;
     bool ok = true;
@@ -309,7 +319,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
       float c = rs;
       if constexpr (Q8) {
         if (np == 1) {
-          c *= ti.ks[0];
+          c = fmaxf(c * ti.ks[0], kTiny);
         } else {
 #pragma unroll
           for (int j = 0; j < KN; ++j) x[j] *= ti.ks[j >> 4];
@@ -325,7 +335,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
 #pragma unroll
           for (int j = 0; j < KN; ++j)
             if (ti.ks[j >> 4] < 0.f) x[j] = -INFINITY;
-          c = rs * fabsf(np == 1 ? ti.ks[0] : 1.f);
+          c = rs;
         }
       }
       float mx[8];
@@ -348,12 +358,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < KN / 2; ++j) {
-        // (a masked score under a factor of zero is not a number: zero then)
-        float p0 = ex2_approx(fmaf(x[2 * j], c, -mu)), p1 = ex2_approx(fmaf(x[2 * j + 1], c, -mu));
-        if (c == 0.f) {
-          p0 = x[2 * j] == -INFINITY ? 0.f : p0;
-          p1 = x[2 * j + 1] == -INFINITY ? 0.f : p1;
-        }
+        const float p0 = ex2_approx(fmaf(x[2 * j], c, -mu)), p1 = ex2_approx(fmaf(x[2 * j + 1], c, -mu));
         sum[j & 3] += p0 + p1;
         pk[j] = pack2<M>(p0, p1);
       }
@@ -405,7 +410,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
         __syncwarp();
 #pragma unroll 4
         for (int j = 0; j < 32 / RP; ++j) {
-          const int r = 32 * q + j * RP + lane / CH, ch = lane % CH, rr = row0 + r;
+          const int r = 32 * q + j * RP + lane / CH, rr = row0 + r;
           const uint4 v = *reinterpret_cast<const uint4*>(sm + r * (D * 2) + ((ch ^ (r & 7)) << 4));
           if (r < valid)
             *reinterpret_cast<uint4*>(reinterpret_cast<H*>(a.out) + (long long)(it.q0 + rr / G) * a.ldo +
