@@ -137,6 +137,30 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
     tmem_alloc(smem_u32(tmem_slot), TM_COLS);
     tmem_relinquish();
   }
+  // ---- softmax warps: 32 rows of Q each, D / 8 lanes a row, asked for before
+  // the wait for the tensor memory (and all of them before the first is stored)
+  constexpr int CH = D / 8, RP = 32 / CH;
+  const int ch = lane % CH;
+  const bool soft_warp = warp >= 1 && warp <= SOFT_WARPS;
+  uint4 qw[32 / RP];
+  // row, head of the group and token of this lane's first row; the next are RP
+  // rows on each
+  const int r_lane = 32 * (warp & 3) + lane / CH;
+  const int i_first = (row0 + r_lane) / G, g_first = (row0 + r_lane) % G;
+  const int i_step = RP / G, g_step = RP % G;
+  if (soft_warp) {
+    int i = i_first, gh = g_first;
+#pragma unroll
+    for (int j = 0; j < 32 / RP; ++j) {
+      qw[j] = make_uint4(0, 0, 0, 0);
+      if (r_lane + j * RP < valid)
+        qw[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const H*>(a.q) + (long long)(it.q0 + i) * a.ldq +
+                                                (h * G + gh) * D + ch * 8);
+      i += i_step;
+      gh += g_step;
+      if (gh >= G) gh -= G, ++i;
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -219,22 +243,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
     const int q = warp & 3;  // TMEM lane quarter
     const int i = 32 * q + lane;
     const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16);
-    // ---- this warp's 32 rows of Q, D / 8 lanes a row
-    constexpr int CH = D / 8, RP = 32 / CH;
-    const int ch = lane % CH;
-    // (all loads before the first store, which they might alias for all that
-    // the compiler knows)
-    uint4 qw[32 / RP];
-#pragma unroll
-    for (int j = 0; j < 32 / RP; ++j) {
-      const int r = 32 * q + j * RP + lane / CH;
-      qw[j] = make_uint4(0, 0, 0, 0);
-      if (r < valid) {
-        const int rr = row0 + r;
-        qw[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const H*>(a.q) + (long long)(it.q0 + rr / G) * a.ldq +
-                                                (h * G + rr % G) * D + ch * 8);
-      }
-    }
+    // ---- this warp's 32 rows of Q into the operand's layout
 #pragma unroll
     for (int j = 0; j < 32 / RP; ++j) {
       const int r = 32 * q + j * RP + lane / CH;
@@ -408,13 +417,20 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
           }
         }
         __syncwarp();
-#pragma unroll 4
+#pragma unroll
         for (int j = 0; j < 32 / RP; ++j) {
-          const int r = 32 * q + j * RP + lane / CH, rr = row0 + r;
-          const uint4 v = *reinterpret_cast<const uint4*>(sm + r * (D * 2) + ((ch ^ (r & 7)) << 4));
-          if (r < valid)
-            *reinterpret_cast<uint4*>(reinterpret_cast<H*>(a.out) + (long long)(it.q0 + rr / G) * a.ldo +
-                                      (h * G + rr % G) * D + ch * 8) = v;
+          const int r = r_lane + j * RP;
+          qw[j] = *reinterpret_cast<const uint4*>(sm + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+        }
+        int i = i_first, gh = g_first;
+#pragma unroll
+        for (int j = 0; j < 32 / RP; ++j) {
+          if (r_lane + j * RP < valid)
+            *reinterpret_cast<uint4*>(reinterpret_cast<H*>(a.out) + (long long)(it.q0 + i) * a.ldo + (h * G + gh) * D +
+                                      ch * 8) = qw[j];
+          i += i_step;
+          gh += g_step;
+          if (gh >= G) gh -= G, ++i;
         }
       } else {
         float* po = a.ws + (part_at(a, row_tiles, b, h, rt) * n_split + split) * (QM * (D + 2));
