@@ -80,18 +80,6 @@ __device__ __forceinline__ uint32_t e4m3_hi(uint32_t w) {
   return r;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // Where 16-byte chunk ch of row r of a tile lies. The reads below take, at a
 // time, four chunks of two neighbouring rows (keys) or two chunks of rows 0, 2,
 // 4, 6 of eight (values): these permutations give each such set eight

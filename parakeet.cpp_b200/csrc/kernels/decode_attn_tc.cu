@@ -40,16 +40,16 @@ namespace {
 
 constexpr int QM = kTileRows;
 constexpr int KN = 64;
-constexpr int RING = 4;
 constexpr int SOFT_WARPS = 4;
 constexpr int CVT_WARPS = 2;
 constexpr float kRescaleLog2 = 8.0f;
 constexpr float kTiny = 1e-38f;  // the least softmax factor: a masked score (-inf) times zero is not a number
 constexpr uint32_t TM_O = 128, TM_COLS = 256;
 
+constexpr int MAX_RING = 4;  // 64-row tiles of keys or values
 enum : int {
-  B_QREADY = 0, B_RFULL = 1, B_REMPTY = B_RFULL + RING, B_SFULL = B_REMPTY + RING, B_PFULL = B_SFULL + 2,
-  B_PVDONE = B_PFULL + 2, B_INFO = B_PVDONE + 2, B_FINAL = B_INFO + RING, N_BARS = B_FINAL + 1
+  B_QREADY = 0, B_RFULL = 1, B_REMPTY = B_RFULL + MAX_RING, B_SFULL = B_REMPTY + MAX_RING, B_PFULL = B_SFULL + 2,
+  B_PVDONE = B_PFULL + 2, B_INFO = B_PVDONE + 2, B_FINAL = B_INFO + MAX_RING, N_BARS = B_FINAL + 1
 };
 
 // What the converting warps tell the softmax about a tile.
@@ -60,17 +60,24 @@ struct TileInfo {
   int parts;      // 1, or the tile's pages
 };
 
-template <int D>
+// Two CTAs have 113 KB each: with the converting warps' raw codes the ring of
+// 128-column tiles has three places instead of four.
+template <bool Q8, int D>
 struct TilesLayout {
   static constexpr int KB = D / 64;
+  static constexpr int RING = Q8 && D == 128 ? 3 : 4;
+  static constexpr int RAW = Q8 ? (D == 128 ? 3 : 4) : 0;  // a converting warp's tiles of codes, on their way
+  static constexpr int RAW_BYTES = 32 * D + 256;           // 32 rows, then two scales a lane
   static constexpr int Q_BYTES = QM * D * 2;
   static constexpr int T_BYTES = KN * D * 2;
   static constexpr int OFF_RING = Q_BYTES;
-  static constexpr int OFF_FACTOR = OFF_RING + RING * T_BYTES;  // [QM] softmax factors
-  static constexpr int OFF_INFO = OFF_FACTOR + QM * 4;          // [RING] TileInfo
+  static constexpr int OFF_RAW = OFF_RING + RING * T_BYTES;
+  static constexpr int OFF_FACTOR = OFF_RAW + CVT_WARPS * RAW * RAW_BYTES;  // [QM] softmax factors
+  static constexpr int OFF_INFO = OFF_FACTOR + QM * 4;                     // [RING] TileInfo
   static constexpr int OFF_BAR = OFF_INFO + RING * 64;
   static constexpr int OFF_SLOT = OFF_BAR + N_BARS * 8;
   static constexpr int SMEM = OFF_SLOT + 16 + 1024;  // + alignment slack
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs share an SM");
 };
 static_assert(sizeof(TileInfo) <= 64, "the layout gives it 64 bytes");
 
@@ -88,7 +95,8 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
     k_attn_tiles(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const DecodeAttnArgs a,
                  int row_tiles, int n_split) {
   using M = typename std::conditional<Q8, __half, H>::type;
-  using L = TilesLayout<D>;
+  using L = TilesLayout<Q8, D>;
+  constexpr int RING = L::RING;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::OFF_BAR);
@@ -121,17 +129,38 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
   const int t0 = split * per;
   const int nT = max(0, min(n_all, t0 + per) - t0);  // this CTA's tiles: t0, t0 + 1, ...
 
-  if (threadIdx.x == 0) {
+  constexpr int LOAD_WARP = 1 + SOFT_WARPS;  // TMA producer, or the first converting warp
+  // 16-bit keys and values: load n of the ring's order K0 K1 V0 K2 V1 ...
+  int n_load = 0, k_load = 0, v_load = 0;
+  auto load_next = [&](uint32_t leader) {
     if constexpr (!Q8) {
-      prefetch_tmap(&tm_k);
-      prefetch_tmap(&tm_v);
+      const int s = n_load % RING;
+      const bool is_k = k_load < nT && n_load == at_k(k_load);
+      const int t = is_k ? k_load++ : v_load++;
+      const CUtensorMap* map = is_k ? &tm_k : &tm_v;
+      mbar_arrive_expect_tx_if(leader, bar(B_RFULL + s), L::T_BYTES);
+#pragma unroll
+      for (int kb = 0; kb < L::KB; ++kb)
+        tma_load_2d_if(leader, sbase + L::OFF_RING + s * L::T_BYTES + kb * KN * 128, map, bar(B_RFULL + s),
+                       h * D + kb * 64, it.kv0 + (t0 + t) * KN);
+      ++n_load;
     }
-    for (int i = 0; i < N_BARS; ++i) {
+  };
+  uint32_t load_leader = 0;
+  if (warp == LOAD_WARP) {
+    if (lane < N_BARS) {
+      const int i = lane;
       const bool soft = i == B_QREADY || i == B_PFULL || i == B_PFULL + 1;
-      const bool full = i >= B_RFULL && i < B_RFULL + RING;
+      const bool full = i >= B_RFULL && i < B_RFULL + MAX_RING;
       mbar_init(bar(i), soft ? SOFT_WARPS : full && Q8 ? CVT_WARPS : 1);
     }
+    static_assert(N_BARS <= 32, "a lane each");
     fence_barrier_init();
+    __syncwarp();
+    // the first loads need not wait for the other warps
+    load_leader = elect_one();
+    if constexpr (!Q8)
+      while (n_load < min(RING, 2 * nT)) load_next(load_leader);
   }
   if (warp == 0) {
     tmem_alloc(smem_u32(tmem_slot), TM_COLS);
@@ -208,10 +237,10 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
           const int left = vmax - (t0 + t) * KN;
           if (left < KN) {
             uint8_t* vt = sm + L::OFF_RING + (n % RING) * L::T_BYTES;
-            for (int i = lane; i < (KN - left) * 8 * L::KB; i += 32) {
-              const int kb = i / ((KN - left) * 8), j = i % ((KN - left) * 8);
-              *reinterpret_cast<uint4*>(vt + kb * KN * 128 + left * 128 + j * 16) = make_uint4(0, 0, 0, 0);
-            }
+#pragma unroll
+            for (int kb = 0; kb < L::KB; ++kb)
+              for (int at = left * 128 + lane * 16; at < KN * 128; at += 512)
+                *reinterpret_cast<uint4*>(vt + kb * KN * 128 + at) = make_uint4(0, 0, 0, 0);
             fence_proxy_async_smem();
             __syncwarp();
           }
@@ -452,27 +481,14 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
     }
   } else if constexpr (!Q8) {
     // ------------------------------------------------------------------ TMA producer
-    if (nT > 0) {
-      const uint32_t leader = elect_one();
-      const int n_loads = 2 * nT;
-      int n = 0, k = 0, v = 0;
-      for (; n < n_loads; ++n) {
-        const int s = n % RING;
-        if (!wwait(B_REMPTY + s, ((uint32_t)(n / RING) & 1u) ^ 1u)) break;
-        const bool is_k = k < nT && n == at_k(k);
-        const int t = is_k ? k++ : v++;
-        const CUtensorMap* map = is_k ? &tm_k : &tm_v;
-        mbar_arrive_expect_tx_if(leader, bar(B_RFULL + s), L::T_BYTES);
-#pragma unroll
-        for (int kb = 0; kb < L::KB; ++kb)
-          tma_load_2d_if(leader, sbase + L::OFF_RING + s * L::T_BYTES + kb * KN * 128, map, bar(B_RFULL + s),
-                         h * D + kb * 64, it.kv0 + (t0 + t) * KN);
-      }
-      if (n < n_loads) {
-        // a consumer gave up: every copy in flight lands before the CTA exits
-        for (int m = n - RING; m < n; ++m)
-          if (m >= 0) mbar_wait(bar(B_RFULL + m % RING), (uint32_t)(m / RING) & 1u, nullptr, 0);
-      }
+    while (n_load < 2 * nT) {
+      if (!wwait(B_REMPTY + n_load % RING, ((uint32_t)(n_load / RING) & 1u) ^ 1u)) break;
+      load_next(load_leader);
+    }
+    if (n_load < 2 * nT) {
+      // a consumer gave up: every copy in flight lands before the CTA exits
+      for (int m = n_load - RING; m < n_load; ++m)
+        if (m >= 0) mbar_wait(bar(B_RFULL + m % RING), (uint32_t)(m / RING) & 1u, nullptr, 0);
     }
   } else {
     // ------------------------------------------------------------ 8-bit converters
@@ -482,50 +498,66 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
       const Kv8& cc = a.cache;
       const int w = warp - 1 - SOFT_WARPS;
       constexpr int LR = D / 16, RI = 32 / LR, IT = 32 / RI;  // lanes a row, rows an iteration, iterations
+      constexpr int RAW = L::RAW;
       const int r_in = lane / LR, ch = lane % LR;
+      const int shift = __ffs(page) - 1;  // of a page in tokens
+      // a lane's own codes and scales, copied RAW - 1 tiles ahead of their use
+      uint8_t* raw = sm + L::OFF_RAW + w * RAW * L::RAW_BYTES + lane * 16;
+      float* raw_sc = reinterpret_cast<float*>(sm + L::OFF_RAW + w * RAW * L::RAW_BYTES + 32 * D + lane * 8);
       auto page_id = [&](int t) -> int {
-        const int key = (t0 + t) * KN + lane * page;
-        return lane < np && t < nT && key < vmax ? cc.table[(long long)b * cc.table_ld + key / page] : -1;
+        const int key = (t0 + t) * KN + (lane << shift);
+        return lane < np && t < nT && key < vmax ? cc.table[(long long)b * cc.table_ld + (key >> shift)] : -1;
       };
       int id_ahead = page_id(0), id_cur = -1, id_prev = -1;
-      float ks_ahead = 1.f, vs_ahead = 1.f;  // scales of the tile whose keys were asked for last
       int k_asked = 0, v_asked = 0;
-      uint4 ahead[IT];
-      // ask for the codes of the next tile in the ring's order
+      // ask for the codes of load n of the ring's order
       auto ask = [&](int n) {
-        if (n >= 2 * nT) return;
-        const bool is_k = k_asked < nT && n == at_k(k_asked);
-        const int t = is_k ? k_asked++ : v_asked++;
-        if (is_k) {
-          id_prev = id_cur;
-          id_cur = id_ahead;
-          id_ahead = page_id(t + 1);
-          const bool on = id_cur >= 0 && id_cur < cc.n_pages;
-          ks_ahead = on ? cc.k_scale[(long long)id_cur * cc.n_kv_heads + h] : -1.f;
-          vs_ahead = on ? cc.v_scale[(long long)id_cur * cc.n_kv_heads + h] : 1.f;
-        }
-        const int ids = is_k || t == k_asked - 1 ? id_cur : id_prev;
-        const uint8_t* pool = is_k ? cc.k : cc.v;
+        if (n < 2 * nT) {
+          const int st = n % RAW;
+          const bool is_k = k_asked < nT && n == at_k(k_asked);
+          const int t = is_k ? k_asked++ : v_asked++;
+          if (is_k) {
+            id_prev = id_cur;
+            id_cur = id_ahead;
+            id_ahead = page_id(t + 1);
+            float* sc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(raw_sc) + st * L::RAW_BYTES);
+            if (id_cur >= 0 && id_cur < cc.n_pages) {
+              const long long ph = (long long)id_cur * cc.n_kv_heads + h;
+              cp_async4(smem_u32(sc), cc.k_scale + ph);
+              cp_async4(smem_u32(sc + 1), cc.v_scale + ph);
+            } else {
+              sc[0] = -1.f;
+              sc[1] = 1.f;
+            }
+          }
+          const int ids = is_k || t == k_asked - 1 ? id_cur : id_prev;
+          const uint8_t* pool = is_k ? cc.k : cc.v;
+          const uint32_t dst = smem_u32(raw + st * L::RAW_BYTES);
 #pragma unroll
-        for (int j = 0; j < IT; ++j) {
-          const int r = 32 * w + j * RI + r_in, key = (t0 + t) * KN + r;
-          const int id = __shfl_sync(0xffffffffu, ids, np == 1 ? 0 : r / page);
-          ahead[j] = make_uint4(0, 0, 0, 0);
-          if (key < vmax && id >= 0 && id < cc.n_pages)
-            ahead[j] = *reinterpret_cast<const uint4*>(
-                pool + (((long long)id * cc.n_kv_heads + h) * page + key % page) * D + ch * 16);
+          for (int j = 0; j < IT; ++j) {
+            const int r = 32 * w + j * RI + r_in, key = (t0 + t) * KN + r;
+            const int id = __shfl_sync(0xffffffffu, ids, r >> shift);
+            const bool in = key < vmax && id >= 0 && id < cc.n_pages;
+            const uint8_t* src =
+                pool + (((((long long)(in ? id : 0) * cc.n_kv_heads + h) << shift) + (key & (page - 1))) * D + ch * 16);
+            cp_async16(dst + j * 512, src, in ? 16 : 0);
+          }
         }
+        cp_commit();
       };
       int ref = 0, dv_cur = 0, dv_prev = 0, k_done = 0, v_done = 0;  // dv: lane j's page, exponent of its values' factor
-      ask(0);
+#pragma unroll
+      for (int n = 0; n < RAW - 1; ++n) ask(n);
       bool ok = true;
       for (int n = 0; n < 2 * nT && ok; ++n) {
+        cp_wait<RAW - 2>();
         uint4 codes[IT];
+        const int st = n % RAW;
 #pragma unroll
-        for (int j = 0; j < IT; ++j) codes[j] = ahead[j];
-        const float ks = ks_ahead, vs = vs_ahead;
-        const int id_here = id_cur;
-        ask(n + 1);
+        for (int j = 0; j < IT; ++j) codes[j] = *reinterpret_cast<const uint4*>(raw + st * L::RAW_BYTES + j * 512);
+        const float2 sc = *reinterpret_cast<const float2*>(reinterpret_cast<uint8_t*>(raw_sc) + st * L::RAW_BYTES);
+        const float ks = sc.x, vs = sc.y;
+        ask(n + RAW - 1);  // into the place read before this one
         const bool is_k = k_done < nT && n == at_k(k_done);
         const int t = is_k ? k_done++ : v_done++;
         const int s = n % RING;
@@ -533,8 +565,8 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
         int dvs = 0;
         if (is_k) {
           // ---- the tile's scales
-          const bool in = lane < np && (t0 + t) * KN + lane * page < vmax;
-          const bool none = in && (id_here < 0 || id_here >= cc.n_pages);
+          const bool in = lane < np && (t0 + t) * KN + (lane << shift) < vmax;
+          const bool none = in && ks < 0.f;
           if (none) report_error(a.err, DEV_ERR_BAD_SHAPE);
           const int ev = ((__float_as_int(vs) >> 23) & 255) - 127;
           const bool counts = in && !none;
@@ -564,7 +596,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
             dv_cur = 0;
           }
           if (w == 0) {
-            const int j = lane < 4 ? (np == 1 ? 0 : lane * 16 / page) : 0;
+            const int j = lane < 4 ? (lane * 16) >> shift : 0;
             const float ks_j = __shfl_sync(0xffffffffu, ks, j);
             const bool in_j = __shfl_sync(0xffffffffu, (int)in, j);
             TileInfo* ti = info(t);
@@ -596,7 +628,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
                 : "r"(cw[e]));
           }
           if (!is_k) {
-            const int dv = __shfl_sync(0xffffffffu, dvs, np == 1 ? 0 : r / page);
+            const int dv = __shfl_sync(0xffffffffu, dvs, r >> shift);
             if (__any_sync(0xffffffffu, dv != 0)) {
               const __half2 m = __float2half2_rn(pow2i(dv < -24 ? -24 : dv));
 #pragma unroll
@@ -618,6 +650,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_RFULL + s));
       }
+      cp_wait<0>();
     }
   }
 
@@ -629,7 +662,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
 template <typename H, bool Q8, int D>
 cudaError_t launch_tiles(const DecodeAttnArgs& a, int row_tiles, int n_split, cudaStream_t st) {
   auto kern = k_attn_tiles<H, Q8, D>;
-  constexpr int smem = TilesLayout<D>::SMEM;
+  constexpr int smem = TilesLayout<Q8, D>::SMEM;
   static PerDevice once;
   int unused = 0;
   const cudaError_t e = per_device(once, &unused, [&](int, int&) {
