@@ -533,6 +533,14 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
           const int ids = is_k || t == k_asked - 1 ? id_cur : id_prev;
           const uint8_t* pool = is_k ? cc.k : cc.v;
           const uint32_t dst = smem_u32(raw + st * L::RAW_BYTES);
+          const int key0 = (t0 + t) * KN;
+          const int id0 = __shfl_sync(0xffffffffu, ids, 0);
+          if (np == 1 && key0 + KN <= vmax && id0 >= 0 && id0 < cc.n_pages) {
+            // a whole tile of one page
+            const uint8_t* src = pool + (((((long long)id0 * cc.n_kv_heads + h) << shift) + (key0 & (page - 1)) + 32 * w + r_in) * D + ch * 16);
+#pragma unroll
+            for (int j = 0; j < IT; ++j) cp_async16(dst + j * 512, src + j * (RI * D), 16);
+          } else
 #pragma unroll
           for (int j = 0; j < IT; ++j) {
             const int r = 32 * w + j * RI + r_in, key = (t0 + t) * KN + r;
@@ -569,31 +577,43 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
           const bool none = in && ks < 0.f;
           if (none) report_error(a.err, DEV_ERR_BAD_SHAPE);
           const int ev = ((__float_as_int(vs) >> 23) & 255) - 127;
-          const bool counts = in && !none;
-          const int mx = __reduce_max_sync(0xffffffffu, counts ? ev : -1000);
-          const int mn = __reduce_min_sync(0xffffffffu, counts ? ev : 1000);
           float grow = 1.f;  // of part j in lane j
           int parts = 1;
           dv_prev = dv_cur;
-          if (mx == -1000) {  // no page: no values
+          if (np == 1) {
+            const int e0 = __shfl_sync(0xffffffffu, none ? -1000 : ev, 0);
             dv_cur = 0;
-          } else if (t > 0 && mx - ref <= 7 && mn - ref >= -15) {
-            dv_cur = counts ? ev - ref : 0;  // (0: no values there)
-          } else if (mx - mn <= 15) {
-            grow = t > 0 ? pow2i(ref - mx) : 1.f;
-            ref = mx;
-            dv_cur = counts ? ev - ref : 0;
+            if (e0 == -1000) {  // no page: no values
+            } else if (t > 0 && e0 - ref <= 7 && e0 - ref >= -15) {
+              dv_cur = e0 - ref;
+            } else {
+              grow = t > 0 ? pow2i(ref - e0) : 1.f;
+              ref = e0;
+            }
           } else {
-            parts = np;
-            // each counting page under its own reference; from which one O comes
-            // to it: the last counting page before, or the tile before
-            const uint32_t have = __ballot_sync(0xffffffffu, counts);
-            const uint32_t before = have & ((1u << lane) - 1u);
-            const int last = 31 - __clz(have);
-            const int from = __shfl_sync(0xffffffffu, ev, before ? 31 - __clz(before) : 0);
-            grow = !counts ? 1.f : before ? pow2i(from - ev) : t > 0 ? pow2i(ref - ev) : 1.f;
-            ref = __shfl_sync(0xffffffffu, ev, last);
-            dv_cur = 0;
+            const bool counts = in && !none;
+            const int mx = __reduce_max_sync(0xffffffffu, counts ? ev : -1000);
+            const int mn = __reduce_min_sync(0xffffffffu, counts ? ev : 1000);
+            if (mx == -1000) {
+              dv_cur = 0;
+            } else if (t > 0 && mx - ref <= 7 && mn - ref >= -15) {
+              dv_cur = counts ? ev - ref : 0;  // (0: no values there)
+            } else if (mx - mn <= 15) {
+              grow = t > 0 ? pow2i(ref - mx) : 1.f;
+              ref = mx;
+              dv_cur = counts ? ev - ref : 0;
+            } else {
+              // each counting page under its own reference; from which one O
+              // comes to it: the last counting page before, or the tile before
+              parts = np;
+              const uint32_t have = __ballot_sync(0xffffffffu, counts);
+              const uint32_t before = have & ((1u << lane) - 1u);
+              const int last = 31 - __clz(have);
+              const int from = __shfl_sync(0xffffffffu, ev, before ? 31 - __clz(before) : 0);
+              grow = !counts ? 1.f : before ? pow2i(from - ev) : t > 0 ? pow2i(ref - ev) : 1.f;
+              ref = __shfl_sync(0xffffffffu, ev, last);
+              dv_cur = 0;
+            }
           }
           if (w == 0) {
             const int j = lane < 4 ? (lane * 16) >> shift : 0;
@@ -614,38 +634,40 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
         } else {
           dvs = t == k_done - 1 ? dv_cur : dv_prev;
         }
-        uint8_t* tile = sm + L::OFF_RING + s * L::T_BYTES;
+        // codes to f16, 16-byte chunks 2 ch and 2 ch + 1 of the row (the other
+        // one first in the second half of the row: fewer bank conflicts)
+        uint8_t* tile = sm + L::OFF_RING + s * L::T_BYTES + (ch >> 2) * KN * 128 + (32 * w + r_in) * 128;
+        const int c0 = (2 * ch) & 7, flip = (ch >> 2) & 1;
+        auto put = [&](bool scaled) {
 #pragma unroll
-        for (int j = 0; j < IT; ++j) {
-          const int r = 32 * w + j * RI + r_in;
-          const uint32_t cw[4] = {codes[j].x, codes[j].y, codes[j].z, codes[j].w};
-          uint32_t f[8];
+          for (int j = 0; j < IT; ++j) {
+            const int r = 32 * w + j * RI + r_in;
+            const uint32_t cw[4] = {codes[j].x, codes[j].y, codes[j].z, codes[j].w};
+            uint32_t f[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
-                "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-                : "=r"(f[2 * e]), "=r"(f[2 * e + 1])
-                : "r"(cw[e]));
-          }
-          if (!is_k) {
-            const int dv = __shfl_sync(0xffffffffu, dvs, r >> shift);
-            if (__any_sync(0xffffffffu, dv != 0)) {
-              const __half2 m = __float2half2_rn(pow2i(dv < -24 ? -24 : dv));
+            for (int e = 0; e < 4; ++e)
+              asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+                  "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+                  : "=r"(f[2 * e]), "=r"(f[2 * e + 1])
+                  : "r"(cw[e]));
+            if (scaled) {
+              const __half2 m = __float2half2_rn(pow2i(__shfl_sync(0xffffffffu, dvs, r >> shift)));
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 __half2 y = __hmul2(*reinterpret_cast<__half2*>(&f[e]), m);
                 f[e] = *reinterpret_cast<uint32_t*>(&y);
               }
             }
+            const uint4 lo = make_uint4(f[0], f[1], f[2], f[3]), hi = make_uint4(f[4], f[5], f[6], f[7]);
+            uint8_t* row = tile + j * RI * 128;
+            *reinterpret_cast<uint4*>(row + (((c0 + flip) ^ (r & 7)) << 4)) = flip ? hi : lo;
+            *reinterpret_cast<uint4*>(row + (((c0 + 1 - flip) ^ (r & 7)) << 4)) = flip ? lo : hi;
           }
-          // 16-byte chunks 2 ch and 2 ch + 1 of the row (the other one first
-          // in the second half of the row: fewer bank conflicts)
-          uint8_t* row = tile + (ch >> 2) * KN * 128 + r * 128;
-          const int c0 = (2 * ch) & 7, flip = (ch >> 2) & 1;
-          const uint4 lo = make_uint4(f[0], f[1], f[2], f[3]), hi = make_uint4(f[4], f[5], f[6], f[7]);
-          *reinterpret_cast<uint4*>(row + (((c0 + flip) ^ (r & 7)) << 4)) = flip ? hi : lo;
-          *reinterpret_cast<uint4*>(row + (((c0 + 1 - flip) ^ (r & 7)) << 4)) = flip ? lo : hi;
-        }
+        };
+        if (!is_k && __any_sync(0xffffffffu, dvs != 0))
+          put(true);
+        else
+          put(false);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_RFULL + s));
