@@ -677,8 +677,9 @@ Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, 
     p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
     p.blocks = (long long)n_items * n_kv_heads * p.row_tiles;
     p.warps = 0;
-    // two CTAs run on an SM: parts of at least 512 keys until all have one
-    const long long want = (2LL * kSms) / (p.blocks > 0 ? p.blocks : 1), most = (max_kv + 511) / 512;
+    // parts of at least 512 keys, enough for two rounds of the two CTAs that
+    // run on an SM (lengths differ)
+    const long long want = (4LL * kSms + p.blocks - 1) / (p.blocks > 0 ? p.blocks : 1), most = (max_kv + 511) / 512;
     const long long n = want < most ? want : most;
     p.n_split = n < 1 ? 1 : n > 64 ? 64 : (int)n;
     return p;
