@@ -66,13 +66,14 @@ template <bool Q8, int D>
 struct TilesLayout {
   static constexpr int KB = D / 64;
   static constexpr int RING = Q8 && D == 128 ? 3 : 4;
-  static constexpr int RAW = Q8 ? (D == 128 ? 3 : 4) : 0;  // a converting warp's tiles of codes, on their way
-  static constexpr int RAW_BYTES = 32 * D + 256;           // 32 rows, then two scales a lane
+  static constexpr int RAW = D == 128 ? 1 : 2;               // tiles of keys, and of values, whose codes are on their way
+  static constexpr int ROWS = KN / CVT_WARPS;                // of a tile, for each converting warp
+  static constexpr int RAW_BYTES = 2 * ROWS * D + 256;       // their codes (keys, values), then two scales a lane
   static constexpr int Q_BYTES = QM * D * 2;
   static constexpr int T_BYTES = KN * D * 2;
   static constexpr int OFF_RING = Q_BYTES;
   static constexpr int OFF_RAW = OFF_RING + RING * T_BYTES;
-  static constexpr int OFF_FACTOR = OFF_RAW + CVT_WARPS * RAW * RAW_BYTES;  // [QM] softmax factors
+  static constexpr int OFF_FACTOR = OFF_RAW + (Q8 ? CVT_WARPS * RAW * RAW_BYTES : 0);  // [QM] softmax factors
   static constexpr int OFF_INFO = OFF_FACTOR + QM * 4;                     // [RING] TileInfo
   static constexpr int OFF_BAR = OFF_INFO + RING * 64;
   static constexpr int OFF_SLOT = OFF_BAR + N_BARS * 8;
@@ -492,86 +493,130 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
     }
   } else {
     // ------------------------------------------------------------ 8-bit converters
-    // Each of the two warps takes 32 of a tile's 64 rows, and both keep the
+    // Each of the warps takes its share of a tile's 64 rows, and all keep the
     // same account of pages and scales (lane j < np: the tile's page j).
     if constexpr (Q8) {
       const Kv8& cc = a.cache;
       const int w = warp - 1 - SOFT_WARPS;
-      constexpr int LR = D / 16, RI = 32 / LR, IT = 32 / RI;  // lanes a row, rows an iteration, iterations
+      constexpr int ROWS = L::ROWS, LR = D / 16, RI = 32 / LR, IT = ROWS / RI;  // lanes a row, rows an iteration, iterations
       constexpr int RAW = L::RAW;
       const int r_in = lane / LR, ch = lane % LR;
       const int shift = __ffs(page) - 1;  // of a page in tokens
-      // a lane's own codes and scales, copied RAW - 1 tiles ahead of their use
+      // a lane's own codes and scales, copied RAW tiles ahead of their use
       uint8_t* raw = sm + L::OFF_RAW + w * RAW * L::RAW_BYTES + lane * 16;
-      float* raw_sc = reinterpret_cast<float*>(sm + L::OFF_RAW + w * RAW * L::RAW_BYTES + 32 * D + lane * 8);
-      auto page_id = [&](int t) -> int {
+      uint8_t* raw_sc = sm + L::OFF_RAW + w * RAW * L::RAW_BYTES + 2 * ROWS * D + lane * 8;
+      const int row_first = ROWS * w + r_in;  // this lane's rows of a tile: it, + RI, ...
+      auto page_id = [&](int t) -> int {      // lane j: the tile's page j
         const int key = (t0 + t) * KN + (lane << shift);
         return lane < np && t < nT && key < vmax ? cc.table[(long long)b * cc.table_ld + (key >> shift)] : -1;
       };
-      int id_ahead = page_id(0), id_cur = -1, id_prev = -1;
-      int k_asked = 0, v_asked = 0;
-      // ask for the codes of load n of the ring's order
-      auto ask = [&](int n) {
-        if (n < 2 * nT) {
-          const int st = n % RAW;
-          const bool is_k = k_asked < nT && n == at_k(k_asked);
-          const int t = is_k ? k_asked++ : v_asked++;
-          if (is_k) {
-            id_prev = id_cur;
-            id_cur = id_ahead;
-            id_ahead = page_id(t + 1);
-            float* sc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(raw_sc) + st * L::RAW_BYTES);
-            if (id_cur >= 0 && id_cur < cc.n_pages) {
-              const long long ph = (long long)id_cur * cc.n_kv_heads + h;
-              cp_async4(smem_u32(sc), cc.k_scale + ph);
-              cp_async4(smem_u32(sc + 1), cc.v_scale + ph);
-            } else {
-              sc[0] = -1.f;
-              sc[1] = 1.f;
-            }
-          }
-          const int ids = is_k || t == k_asked - 1 ? id_cur : id_prev;
-          const uint8_t* pool = is_k ? cc.k : cc.v;
-          const uint32_t dst = smem_u32(raw + st * L::RAW_BYTES);
-          const int key0 = (t0 + t) * KN;
-          const int id0 = __shfl_sync(0xffffffffu, ids, 0);
-          if (np == 1 && key0 + KN <= vmax && id0 >= 0 && id0 < cc.n_pages) {
-            // a whole tile of one page
-            const uint8_t* src = pool + (((((long long)id0 * cc.n_kv_heads + h) << shift) + (key0 & (page - 1)) + 32 * w + r_in) * D + ch * 16);
+      // ask for a tile's codes, keys (x = 0) or values
+      auto ask = [&](int x, int t, int ids) {
+        if (t < 0 || t >= nT) return;
+        const uint8_t* pool = x ? cc.v : cc.k;
+        const uint32_t dst = smem_u32(raw) + (t % RAW) * L::RAW_BYTES + x * ROWS * D;
+        const int key0 = (t0 + t) * KN;
+        const int id0 = __shfl_sync(0xffffffffu, ids, 0);
+        if (np == 1 && key0 + KN <= vmax && id0 >= 0 && id0 < cc.n_pages) {  // a whole tile of one page
+          const uint8_t* src =
+              pool + ((((long long)id0 * cc.n_kv_heads + h) << shift) + (key0 & (page - 1)) + row_first) * D + ch * 16;
 #pragma unroll
-            for (int j = 0; j < IT; ++j) cp_async16(dst + j * 512, src + j * (RI * D), 16);
-          } else
+          for (int j = 0; j < IT; ++j) cp_async16(dst + j * 512, src + j * (RI * D), 16);
+        } else {
 #pragma unroll
           for (int j = 0; j < IT; ++j) {
-            const int r = 32 * w + j * RI + r_in, key = (t0 + t) * KN + r;
+            const int r = row_first + j * RI, key = key0 + r;
             const int id = __shfl_sync(0xffffffffu, ids, r >> shift);
             const bool in = key < vmax && id >= 0 && id < cc.n_pages;
             const uint8_t* src =
-                pool + (((((long long)(in ? id : 0) * cc.n_kv_heads + h) << shift) + (key & (page - 1))) * D + ch * 16);
+                pool + ((((long long)(in ? id : 0) * cc.n_kv_heads + h) << shift) + (key & (page - 1))) * D + ch * 16;
             cp_async16(dst + j * 512, src, in ? 16 : 0);
           }
         }
-        cp_commit();
       };
-      int ref = 0, dv_cur = 0, dv_prev = 0, k_done = 0, v_done = 0;  // dv: lane j's page, exponent of its values' factor
+      auto ask_scales = [&](int t, int ids) {
+        if (t >= nT) return;
+        uint8_t* sc = raw_sc + (t % RAW) * L::RAW_BYTES;
+        if (ids >= 0 && ids < cc.n_pages) {
+          const long long ph = (long long)ids * cc.n_kv_heads + h;
+          cp_async4(smem_u32(sc), cc.k_scale + ph);
+          cp_async4(smem_u32(sc) + 4, cc.v_scale + ph);
+        } else {
+          *reinterpret_cast<float2*>(sc) = make_float2(-1.f, 1.f);
+        }
+      };
+      // codes to f16 into the ring's next place: 16-byte chunks 2 ch and
+      // 2 ch + 1 of the row (the other one first in the second half of the
+      // row: fewer bank conflicts), times 2^dv of the row's page
+      int place = 0;
+      uint32_t lap = 1;  // parity of the place's last release
+      const int c0 = (2 * ch) & 7, flip = (ch >> 2) & 1;
+      auto put = [&](const uint4 (&codes)[IT], int dv) -> bool {
+        if (!wwait(B_REMPTY + place, lap)) return false;
+        uint8_t* tile = sm + L::OFF_RING + place * L::T_BYTES + (ch >> 2) * KN * 128 + row_first * 128;
+        const bool scaled = __any_sync(0xffffffffu, dv != 0);
 #pragma unroll
-      for (int n = 0; n < RAW - 1; ++n) ask(n);
+        for (int j = 0; j < IT; ++j) {
+          const int r = row_first + j * RI;
+          const uint32_t cw[4] = {codes[j].x, codes[j].y, codes[j].z, codes[j].w};
+          uint32_t f[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+                "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+                : "=r"(f[2 * e]), "=r"(f[2 * e + 1])
+                : "r"(cw[e]));
+          if (scaled) {
+            const __half2 m = __float2half2_rn(pow2i(__shfl_sync(0xffffffffu, dv, r >> shift)));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              __half2 y = __hmul2(*reinterpret_cast<__half2*>(&f[e]), m);
+              f[e] = *reinterpret_cast<uint32_t*>(&y);
+            }
+          }
+          const uint4 lo = make_uint4(f[0], f[1], f[2], f[3]), hi = make_uint4(f[4], f[5], f[6], f[7]);
+          uint8_t* row = tile + j * RI * 128;
+          *reinterpret_cast<uint4*>(row + (((c0 + flip) ^ (r & 7)) << 4)) = flip ? hi : lo;
+          *reinterpret_cast<uint4*>(row + (((c0 + 1 - flip) ^ (r & 7)) << 4)) = flip ? lo : hi;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_RFULL + place));
+        if (++place == RING) place = 0, lap ^= 1u;
+        return true;
+      };
+      // step t turns keys t and values t - 1, and asks for keys t + RAW and
+      // values t + RAW - 1
+      int id_k = page_id(0), id_v = -1;  // pages of the tiles asked for next
+      int ref = 0, dv_cur = 0, dv_prev = 0;  // exponents of the values' factors, lane j: page j of tiles t, t - 1
       bool ok = true;
-      for (int n = 0; n < 2 * nT && ok; ++n) {
-        cp_wait<RAW - 2>();
-        uint4 codes[IT];
-        const int st = n % RAW;
+#pragma unroll 1
+      for (int t = -RAW; t <= nT && ok; ++t) {
+        uint4 kc[IT], vc[IT];
+        float ks = 1.f, vs = 1.f;
+        if (t >= 0) {
+          cp_wait<RAW - 1>();
+          const uint8_t* kr = raw + (t % RAW) * L::RAW_BYTES;
+          const uint8_t* vr = raw + ((t + RAW - 1) % RAW) * L::RAW_BYTES + ROWS * D;
 #pragma unroll
-        for (int j = 0; j < IT; ++j) codes[j] = *reinterpret_cast<const uint4*>(raw + st * L::RAW_BYTES + j * 512);
-        const float2 sc = *reinterpret_cast<const float2*>(reinterpret_cast<uint8_t*>(raw_sc) + st * L::RAW_BYTES);
-        const float ks = sc.x, vs = sc.y;
-        ask(n + RAW - 1);  // into the place read before this one
-        const bool is_k = k_done < nT && n == at_k(k_done);
-        const int t = is_k ? k_done++ : v_done++;
-        const int s = n % RING;
-        if (!(ok = wwait(B_REMPTY + s, ((uint32_t)(n / RING) & 1u) ^ 1u))) break;
-        int dvs = 0;
-        if (is_k) {
+          for (int j = 0; j < IT; ++j) {
+            kc[j] = *reinterpret_cast<const uint4*>(kr + j * 512);
+            vc[j] = *reinterpret_cast<const uint4*>(vr + j * 512);
+          }
+          const float2 sc = *reinterpret_cast<const float2*>(raw_sc + (t % RAW) * L::RAW_BYTES);
+          ks = sc.x;
+          vs = sc.y;
+        }
+        const int id_next = page_id(t + RAW + 1);
+        ask(0, t + RAW, id_k);
+        ask_scales(t + RAW, id_k);
+        ask(1, t + RAW - 1, id_v);
+        cp_commit();
+        id_v = id_k;
+        id_k = id_next;
+        if (t < 0) continue;
+        dv_prev = dv_cur;
+        if (t < nT) {
           // ---- the tile's scales
           const bool in = lane < np && (t0 + t) * KN + (lane << shift) < vmax;
           const bool none = in && ks < 0.f;
@@ -579,7 +624,6 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
           const int ev = ((__float_as_int(vs) >> 23) & 255) - 127;
           float grow = 1.f;  // of part j in lane j
           int parts = 1;
-          dv_prev = dv_cur;
           if (np == 1) {
             const int e0 = __shfl_sync(0xffffffffu, none ? -1000 : ev, 0);
             dv_cur = 0;
@@ -616,9 +660,11 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
             }
           }
           if (w == 0) {
+            // (info t's place was read before values t - RING + 1 were released)
             const int j = lane < 4 ? (lane * 16) >> shift : 0;
             const float ks_j = __shfl_sync(0xffffffffu, ks, j);
             const bool in_j = __shfl_sync(0xffffffffu, (int)in, j);
+            if (!(ok = wwait(B_REMPTY + place, lap))) break;
             TileInfo* ti = info(t);
             if (lane < 4) {
               ti->ks[lane] = in_j ? ks_j : 1.f;  // (keys behind the last are masked)
@@ -631,46 +677,9 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(B_INFO + t % RING));
           }
-        } else {
-          dvs = t == k_done - 1 ? dv_cur : dv_prev;
+          if (!(ok = put(kc, 0))) break;
         }
-        // codes to f16, 16-byte chunks 2 ch and 2 ch + 1 of the row (the other
-        // one first in the second half of the row: fewer bank conflicts)
-        uint8_t* tile = sm + L::OFF_RING + s * L::T_BYTES + (ch >> 2) * KN * 128 + (32 * w + r_in) * 128;
-        const int c0 = (2 * ch) & 7, flip = (ch >> 2) & 1;
-        auto put = [&](bool scaled) {
-#pragma unroll
-          for (int j = 0; j < IT; ++j) {
-            const int r = 32 * w + j * RI + r_in;
-            const uint32_t cw[4] = {codes[j].x, codes[j].y, codes[j].z, codes[j].w};
-            uint32_t f[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
-                  "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-                  : "=r"(f[2 * e]), "=r"(f[2 * e + 1])
-                  : "r"(cw[e]));
-            if (scaled) {
-              const __half2 m = __float2half2_rn(pow2i(__shfl_sync(0xffffffffu, dvs, r >> shift)));
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                __half2 y = __hmul2(*reinterpret_cast<__half2*>(&f[e]), m);
-                f[e] = *reinterpret_cast<uint32_t*>(&y);
-              }
-            }
-            const uint4 lo = make_uint4(f[0], f[1], f[2], f[3]), hi = make_uint4(f[4], f[5], f[6], f[7]);
-            uint8_t* row = tile + j * RI * 128;
-            *reinterpret_cast<uint4*>(row + (((c0 + flip) ^ (r & 7)) << 4)) = flip ? hi : lo;
-            *reinterpret_cast<uint4*>(row + (((c0 + 1 - flip) ^ (r & 7)) << 4)) = flip ? lo : hi;
-          }
-        };
-        if (!is_k && __any_sync(0xffffffffu, dvs != 0))
-          put(true);
-        else
-          put(false);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_RFULL + s));
+        if (t > 0) ok = put(vc, dv_prev);
       }
       cp_wait<0>();
     }
