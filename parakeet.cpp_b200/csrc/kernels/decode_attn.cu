@@ -80,6 +80,21 @@ __device__ __forceinline__ uint32_t e4m3_hi(uint32_t w) {
   return r;
 }
 
+// from the shared memory of a CTA of the cluster
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 // Where 16-byte chunk ch of row r of a tile lies. The reads below take, at a
 // time, four chunks of two neighbouring rows (keys) or two chunks of rows 0, 2,
 // 4, 6 of eight (values): these permutations give each such set eight
@@ -111,7 +126,7 @@ struct RowsLayout {
 // H: type of q and out; Q8: 8-bit cache, else keys and values of type H; W
 // warps share the CTA's part of the keys; NB blocks of 8 query rows.
 template <typename H, bool Q8, int D, int WT, int W, int NB>
-__global__ void __launch_bounds__(32 * W, NB == 1 ? 12 / W : 8 / W) k_attn_rows(const DecodeAttnArgs a, int row_tiles, int n_split) {
+__global__ void __launch_bounds__(32 * W, NB == 1 ? 12 / W : 8 / W) k_attn_rows(const DecodeAttnArgs a, int row_tiles, int n_split, int clustered) {
   using M = typename std::conditional<Q8, __half, H>::type;  // type of the products
   constexpr int RB = Q8 ? D : 2 * D;                         // bytes of a row
   constexpr int KC = RB / 64;                                // 16-byte reads of a key row, per thread
@@ -536,26 +551,12 @@ __global__ void __launch_bounds__(32 * W, NB == 1 ? 12 / W : 8 / W) k_attn_rows(
     H* op = reinterpret_cast<H*>(a.out) + (long long)(it.q0 + row / G) * a.ldo + (h * G + row % G) * D + dim;
     *reinterpret_cast<uint2*>(op) = make_uint2(pack2<H>(v.x, v.y), pack2<H>(v.z, v.w));
   };
-  if constexpr (W == 1) {
-    if (n_split == 1) {
-      each([&](int nb, int x, int dim, float4 v) {
-        const int r = nb * 8 + 2 * c + x;
-        const float inv = l[nb][x] == 0.f ? 0.f : 1.f / l[nb][x];  // no key seen: zeros
-        if (r < valid) store_out(r, dim, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-      });
-    } else {
-      each([&](int nb, int x, int dim, float4 v) {
-        const int r = nb * 8 + 2 * c + x;
-        if (r < valid) *reinterpret_cast<float4*>(po + r * D + dim) = v;
-      });
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int r = nb * 8 + 2 * c + x;
-          if (g == 0 && r < valid) *reinterpret_cast<float2*>(po + R * D + 2 * r) = make_float2(m[nb][x], l[nb][x]);
-        }
-    }
+  if constexpr (W == 1) {  // (alone with its rows)
+    each([&](int nb, int x, int dim, float4 v) {
+      const int r = nb * 8 + 2 * c + x;
+      const float inv = l[nb][x] == 0.f ? 0.f : 1.f / l[nb][x];  // no key seen: zeros
+      if (r < valid) store_out(r, dim, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    });
   } else {
     // ---- join the warps, in the rings' memory
     cp_wait<0>();
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(32 * W, NB == 1 ? 12 / W : 8 / W) k_attn_rows(
     constexpr int LD = D + 4;
     float* s_o = reinterpret_cast<float*>(smem);  // [W][R][LD]
     float* s_ml = s_o + W * R * LD;               // [W][R][2]
-    static_assert((W * R * (LD + 2)) * 4 <= W * L::kWarp, "the join fits the rings");
+    float* s_p = s_ml + W * R * 2;                // [R][LD] this CTA's sums, then [R][2]
     each([&](int nb, int x, int dim, float4 v) {
       *reinterpret_cast<float4*>(s_o + (warp * R + nb * 8 + 2 * c + x) * LD + dim) = v;
     });
@@ -595,22 +596,52 @@ __global__ void __launch_bounds__(32 * W, NB == 1 ? 12 / W : 8 / W) k_attn_rows(
         const float inv = ll == 0.f ? 0.f : 1.f / ll;
         store_out(r, d4, make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv));
       } else {
-        *reinterpret_cast<float4*>(po + r * D + d4) = make_float4(x[0], x[1], x[2], x[3]);
-        if (d4 == 0) *reinterpret_cast<float2*>(po + R * D + 2 * r) = make_float2(mm, ll);
+        float* to = clustered ? s_p + r * LD : po + r * D;
+        *reinterpret_cast<float4*>(to + d4) = make_float4(x[0], x[1], x[2], x[3]);
+        if (d4 == 0) *reinterpret_cast<float2*>(clustered ? s_p + R * LD + 2 * r : po + R * D + 2 * r) = make_float2(mm, ll);
       }
+    }
+    if (clustered) {
+      // ---- the parts are the CTAs of a cluster: join them through distributed
+      // shared memory, four columns a thread
+      cluster_sync();
+      const uint32_t base_s = smem_u32(s_p), ml_s = smem_u32(s_p + R * LD);
+      for (int idx = split * 32 * W + threadIdx.x; idx < valid * (D / 4); idx += n_split * 32 * W) {
+        const int r = idx / (D / 4), d4 = idx % (D / 4) * 4;
+        float mm = -INFINITY;
+        for (int s = 0; s < n_split; ++s) mm = fmaxf(mm, ld_cluster2(mapa_shared(ml_s + 8 * r, s)).x);
+        const float base = mm == -INFINITY ? 0.f : mm;
+        float ll = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < n_split; ++s) {
+          const float2 ml = ld_cluster2(mapa_shared(ml_s + 8 * r, s));
+          const float4 v = ld_cluster4(mapa_shared(base_s + (r * LD + d4) * 4, s));
+          const float f = ex2_approx(ml.x - base);
+          ll = fmaf(ml.y, f, ll);
+          x[0] = fmaf(v.x, f, x[0]);
+          x[1] = fmaf(v.y, f, x[1]);
+          x[2] = fmaf(v.z, f, x[2]);
+          x[3] = fmaf(v.w, f, x[3]);
+        }
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        store_out(r, d4, make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv));
+      }
+      cluster_sync();  // every part has been read
     }
   }
 }
 
-// Joins the parts of one row: o = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).
-// Four warps take every fourth part each (a part is a read that depends on
-// nothing), then add up.
-template <typename H, bool Q8, int D, int R>
+// Joins the parts of a row: o = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).
+// P warps a row, each taking every P-th part (a part is a read that depends on
+// nothing): four for the few rows of k_attn_rows, whose parts are many, one for
+// the 128-row tiles.
+template <typename H, bool Q8, int D, int R, int P>
 __global__ void __launch_bounds__(128) k_attn_join(const DecodeAttnArgs a, int row_tiles, int n_split) {
   __shared__ float s_x[4][D], s_l[4];
+  constexpr int RC = 4 / P;  // rows of a CTA
   const int G = a.n_heads / a.n_kv_heads;
-  const int r = blockIdx.x % R;
-  int rest = blockIdx.x / R;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.x % (R / RC) * RC + warp / P;
+  int rest = blockIdx.x / (R / RC);
   const int rt = rest % row_tiles;
   rest /= row_tiles;
   const int h = rest % a.n_kv_heads, b = rest / a.n_kv_heads;
@@ -618,7 +649,7 @@ __global__ void __launch_bounds__(128) k_attn_join(const DecodeAttnArgs a, int r
   pdl_trigger();
   const Item it = load_item<Q8>(a, b);
   if (!it.ok) return;
-  const int row = rt * R + r, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = rt * R + r;
   if (row >= it.n * G) return;
   constexpr int PS = R * (D + 2);  // floats of a part
   const float* p = a.ws + part_at(a, row_tiles, b, h, rt) * n_split * PS;
@@ -631,27 +662,29 @@ __global__ void __launch_bounds__(128) k_attn_join(const DecodeAttnArgs a, int r
   constexpr int V = D / 32;  // columns of a lane
   float x[V] = {}, l = 0.f;
 #pragma unroll 4
-  for (int s = warp; s < n_split; s += 4) {
+  for (int s = warp % P; s < n_split; s += P) {
     const float2 ml = *reinterpret_cast<const float2*>(p + s * PS + R * D + 2 * r);
     if (ml.x == -INFINITY && ml.y == 0.f) continue;  // a part without keys leaves its sums unwritten
     const float f = ex2_approx(ml.x - base);
     l = fmaf(ml.y, f, l);
 #pragma unroll
-    for (int v = 0; v < V; ++v) x[v] = fmaf(p[s * PS + r * D + v * 32 + lane], f, x[v]);
+    for (int v = 0; v < V; ++v) x[v] = fmaf(p[s * PS + r * D + V * lane + v], f, x[v]);
   }
+  if constexpr (P > 1) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) s_x[warp][v * 32 + lane] = x[v];
-  if (lane == 0) s_l[warp] = l;
-  __syncthreads();
-  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (threadIdx.x < D / 2) {
-    const int d = 2 * threadIdx.x;
-    const float y0 = (s_x[0][d] + s_x[1][d]) + (s_x[2][d] + s_x[3][d]);
-    const float y1 = (s_x[0][d + 1] + s_x[1][d + 1]) + (s_x[2][d + 1] + s_x[3][d + 1]);
-    H* op = reinterpret_cast<H*>(a.out) + (long long)(it.q0 + row / G) * a.ldo + (h * G + row % G) * D + d;
-    *reinterpret_cast<uint32_t*>(op) = pack2<H>(y0 * inv, y1 * inv);
+    for (int v = 0; v < V; ++v) s_x[warp][V * lane + v] = x[v];
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    if (warp > 0) return;
+    l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      x[v] = (s_x[0][V * lane + v] + s_x[1][V * lane + v]) + (s_x[2][V * lane + v] + s_x[3][V * lane + v]);
   }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  H* op = reinterpret_cast<H*>(a.out) + (long long)(it.q0 + row / G) * a.ldo + (h * G + row % G) * D + V * lane;
+#pragma unroll
+  for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t*>(op + v) = pack2<H>(x[v] * inv, x[v + 1] * inv);
 }
 
 // How a call is cut. (tiles: false for what the tcgen05 kernel cannot describe,
@@ -660,13 +693,17 @@ __global__ void __launch_bounds__(128) k_attn_join(const DecodeAttnArgs a, int r
 //    (decode_attn_tc.cu), the keys in parts where there are few tiles.
 //  - Blocks of 8 rows, or of 16 where an item has more: they share one read of
 //    the keys.
-//  - Many blocks: a warp takes one alone (CTAs of one warp, no join).
-//  - Else four warps share a part, and the keys are cut into as many parts as
-//    give about six CTAs an SM (lengths differ; two run at a time), of at
-//    least 128 keys.
+//  - Twelve warps run on an SM. Many blocks: a warp takes one alone (CTAs of
+//    one warp, no join); fewer: four warps share one.
+//  - Still fewer: the keys are cut into parts of at least 128, one for each CTA
+//    of a cluster, which joins them: one launch and no workspace.
+//  - Where that leaves SMs without work and the parts are long, into more
+//    parts, about six CTAs an SM (lengths differ; three run at a time), joined
+//    by a second kernel.
 constexpr int kFewRows = 32;
 struct Plan {
   int rows, row_tiles, warps, n_split;  // warps 0: the tcgen05 kernel
+  bool clustered;                       // the parts are joined in a cluster
   long long blocks;
 };
 Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, bool tiles = true) {
@@ -677,9 +714,10 @@ Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, 
     p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
     p.blocks = (long long)n_items * n_kv_heads * p.row_tiles;
     p.warps = 0;
-    // parts of at least 512 keys, enough for two rounds of the two CTAs that
-    // run on an SM (lengths differ)
-    const long long want = (4LL * kSms + p.blocks - 1) / (p.blocks > 0 ? p.blocks : 1), most = (max_kv + 511) / 512;
+    p.clustered = false;
+    // parts of at least 512 keys (a part costs as much as six more tiles),
+    // until two CTAs run on every SM
+    const long long want = (2LL * kSms + p.blocks - 1) / (p.blocks > 0 ? p.blocks : 1), most = max_kv / 512;
     const long long n = want < most ? want : most;
     p.n_split = n < 1 ? 1 : n > 64 ? 64 : (int)n;
     return p;
@@ -687,14 +725,17 @@ Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, 
   p.rows = rows <= 8 ? 8 : 16;
   p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
   p.blocks = (long long)n_items * n_kv_heads * p.row_tiles;
-  p.warps = 1;
+  constexpr long long slots = 12LL * kSms;
+  p.warps = 2 * p.blocks > slots ? 1 : 4;
   p.n_split = 1;
-  if (p.blocks < 8LL * kSms && tiles) {
-    p.warps = 4;
-    const long long want = (6LL * kSms + p.blocks - 1) / (p.blocks > 0 ? p.blocks : 1);
-    const long long most = (max_kv + 127) / 128;
-    const long long n = want < most ? want : most;
-    p.n_split = n < 1 ? 1 : n > 64 ? 64 : (int)n;
+  p.clustered = false;
+  if (p.warps == 4 && tiles && p.blocks > 0) {
+    const long long most = (max_kv + 127) / 128, want = 2 * slots / (4 * p.blocks);  // two rounds of CTAs
+    const long long n0 = want < most ? want : most;
+    p.clustered = n0 <= 8 || max_kv <= 8 * 1024;
+    const long long n = p.clustered && n0 > 8 ? 8 : n0 > 64 ? 64 : n0;
+    p.n_split = n < 1 ? 1 : (int)n;
+    p.clustered = p.clustered && p.n_split > 1;
   }
   return p;
 }
@@ -702,16 +743,31 @@ Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, 
 template <typename H, bool Q8, int D, int WT, int W, int NB>
 cudaError_t launch_w(const DecodeAttnArgs& a, const Plan& p, cudaStream_t st) {
   auto kern = k_attn_rows<H, Q8, D, WT, W, NB>;
-  constexpr int smem = W * RowsLayout<Q8 ? D : 2 * D, WT, NB>::kWarp;
+  // the rings, and in their place the join of the warps
+  constexpr int rings = W * RowsLayout<Q8 ? D : 2 * D, WT, NB>::kWarp, join = (W + 1) * 8 * NB * (D + 6) * 4;
+  constexpr int smem = W > 1 && join > rings ? join : rings;
   static PerDevice once;
   int unused = 0;
   cudaError_t e = per_device(once, &unused, [&](int, int&) {
     return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kern, dim3((unsigned)(p.blocks * p.n_split)), dim3(32 * W), smem, st, a, p.row_tiles, p.n_split);
-  if (e != cudaSuccess || p.n_split == 1) return e;
-  return launch_pdl(k_attn_join<H, Q8, D, 8 * NB>, dim3((unsigned)(p.blocks * 8 * NB)), dim3(128), 0, st, a, p.row_tiles,
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.blocks * p.n_split));
+  cfg.blockDim = dim3(32 * W);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = p.n_split;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.clustered ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, a, p.row_tiles, p.n_split, p.clustered ? 1 : 0);
+  if (e != cudaSuccess || p.n_split == 1 || p.clustered) return e;
+  return launch_pdl(k_attn_join<H, Q8, D, 8 * NB, 4>, dim3((unsigned)(p.blocks * 8 * NB)), dim3(128), 0, st, a, p.row_tiles,
                     p.n_split);
 }
 
@@ -722,7 +778,7 @@ cudaError_t launch_rows(const DecodeAttnArgs& a, cudaStream_t st) {
   if (p.warps == 0) {
     const cudaError_t e = attn_tiles_launch(a, is_bf16<H>::value, p.row_tiles, p.n_split, st);
     if (e != cudaSuccess || p.n_split == 1) return e;
-    return launch_pdl(k_attn_join<H, Q8, D, kTileRows>, dim3((unsigned)(p.blocks * kTileRows)), dim3(128), 0, st, a,
+    return launch_pdl(k_attn_join<H, Q8, D, kTileRows, 1>, dim3((unsigned)(p.blocks * (kTileRows / 4))), dim3(128), 0, st, a,
                       p.row_tiles, p.n_split);
   }
   if (p.rows == 8)
@@ -744,7 +800,7 @@ cudaError_t launch_h(const DecodeAttnArgs& a, cudaStream_t st) {
 
 size_t decode_attn_ws_bytes(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, int head_dim, bool) {
   const Plan p = plan_rows(n_items, max_q, max_kv, n_heads, n_kv_heads);
-  return p.n_split == 1 ? 0 : (size_t)p.blocks * p.n_split * p.rows * (head_dim + 2) * sizeof(float);
+  return p.n_split == 1 || p.clustered ? 0 : (size_t)p.blocks * p.n_split * p.rows * (head_dim + 2) * sizeof(float);
 }
 
 cudaError_t decode_attn_launch(const DecodeAttnArgs& a, bool bf16, cudaStream_t st) {

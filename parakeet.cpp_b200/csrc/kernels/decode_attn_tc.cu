@@ -86,6 +86,17 @@ static_assert(sizeof(TileInfo) <= 64, "the layout gives it 64 bytes");
 __device__ __forceinline__ int at_k(int t) { return t < 2 ? t : 2 * t - 1; }
 __device__ __forceinline__ int at_v(int t, int n) { return t < n - 2 ? 2 * t + 2 : t == n - 1 ? 2 * n - 1 : 2 * n - 2; }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 __device__ __forceinline__ float pow2i(int e) {
   e = e < -126 ? -126 : e > 127 ? 127 : e;
   return __int_as_float((e + 127) << 23);
@@ -377,15 +388,16 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
           c = rs;
         }
       }
-      float mx[8];
+      // (three-way maxima; a NaN is passed over here and makes its weight one)
+      float mx[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        mx[k] = x[k];
+      for (int k = 0; k < 4; ++k) {
+        mx[k] = max3(x[k], x[4 + k], x[8 + k]);
 #pragma unroll
-        for (int j = 1; j < KN / 8; ++j) mx[k] = fmaxf(mx[k], x[8 * j + k]);
+        for (int j = 12; j < KN - 4; j += 8) mx[k] = max3(mx[k], x[j + k], x[j + 4 + k]);
+        mx[k] = fmaxf(mx[k], x[KN - 4 + k]);
       }
-      const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                             fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * c;
+      const float mt = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * c;
       float alpha = 1.f;
       if (mt > m_used + kRescaleLog2) {
         alpha = ex2_approx(m_used - mt);
@@ -394,14 +406,17 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
       }
       const float mu = m_used == -INFINITY ? 0.f : m_used;
       uint32_t pk[KN / 2];
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint64_t sum[4] = {0, 0, 0, 0};
+      const uint64_t c2 = f2_pack(c, c), mu2 = f2_pack(-mu, -mu);
 #pragma unroll
       for (int j = 0; j < KN / 2; ++j) {
-        const float p0 = ex2_approx(fmaf(x[2 * j], c, -mu)), p1 = ex2_approx(fmaf(x[2 * j + 1], c, -mu));
-        sum[j & 3] += p0 + p1;
+        const float2 y = f2_unpack(ffma2(f2_pack(x[2 * j], x[2 * j + 1]), c2, mu2));
+        const float p0 = ex2_approx(y.x), p1 = ex2_approx(y.y);
+        sum[j & 3] = fadd2(sum[j & 3], f2_pack(p0, p1));
         pk[j] = pack2<M>(p0, p1);
       }
-      lsum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      const float2 total = f2_unpack(fadd2(fadd2(sum[0], sum[1]), fadd2(sum[2], sum[3])));
+      lsum += total.x + total.y;
       tmem_st32(trow + 64u * buf, pk);
       // ---- O: the row's maximum moved, or the reference of the values did
       const int parts = Q8 ? ti.parts : 1;
