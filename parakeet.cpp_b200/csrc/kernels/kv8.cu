@@ -53,14 +53,96 @@ __device__ __forceinline__ uint2 rescale8(uint2 c, float f) {
   return make_uint2(w[0], w[1]);
 }
 
-// One group of T threads (a warp or a CTA) writes one page's new tokens of one
-// head, keys or values: D / 8 vectors of 8 values a token.
-template <typename H, int T>
-__global__ void __launch_bounds__(128) k_kv8_append(const Kv8AppendArgs a, int width, long long units) {
-  constexpr int kGroups = 128 / T;
-  __shared__ float s_max[4];
-  const long long unit = (long long)blockIdx.x * kGroups + threadIdx.x / T;
-  const int lane = threadIdx.x % T;
+// What a page's new tokens are for one sequence, checked against the sizes of
+// the call.
+struct PageShare {
+  int t0, t1;       // its tokens t0 .. t1 - 1 are new; 0 .. t0 - 1 are old
+  long long row;    // row of token t0 among the new ones
+  int id;           // the page
+  bool on;
+};
+__device__ __forceinline__ PageShare page_share(const Kv8AppendArgs& a, int s, int w, bool report) {
+  const Kv8& c = a.c;
+  PageShare p{0, 0, 0, 0, false};
+  const int r0 = a.new_off[s], n = a.new_off[s + 1] - r0, len = a.lens[s];
+  if (n == 0) return p;
+  if (r0 < 0 || n < 0 || n > a.max_new || r0 > a.rows - n || len < n || len > (long long)c.table_ld * c.page) {
+    if (report) report_error(a.err, DEV_ERR_BAD_SHAPE);
+    return p;
+  }
+  const int base = len - n, pg = base / c.page + w;  // tokens before, this share's page
+  if ((long long)pg * c.page >= len) return p;
+  p.id = c.table[(long long)s * c.table_ld + pg];
+  if (p.id < 0 || p.id >= c.n_pages) {
+    if (report) report_error(a.err, DEV_ERR_BAD_SHAPE);
+    return p;
+  }
+  p.t0 = max(base - pg * c.page, 0);
+  p.t1 = min(len - pg * c.page, c.page);
+  p.row = (long long)r0 + (pg * c.page + p.t0 - base);
+  p.on = true;
+  return p;
+}
+
+// The magnitudes of 16-bit floats order as unsigned integers, a NaN above the
+// infinity above the finite values: running maximum of two of them at a time.
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t look8(uint4 raw, uint32_t most) {
+  most = max_u16x2(most, raw.x & 0x7fff7fffu);
+  most = max_u16x2(most, raw.y & 0x7fff7fffu);
+  most = max_u16x2(most, raw.z & 0x7fff7fffu);
+  return max_u16x2(most, raw.w & 0x7fff7fffu);
+}
+template <typename H>
+__device__ __forceinline__ float value16(uint32_t bits) {
+  if constexpr (is_bf16<H>::value)
+    return __uint_as_float(bits << 16);
+  else
+    return __half2float(__ushort_as_half((unsigned short)bits));
+}
+// the bits of infinity
+template <typename H>
+__device__ __forceinline__ uint32_t inf16() { return is_bf16<H>::value ? 0x7f80u : 0x7c00u; }
+// largest finite magnitude of eight values where some are not finite, and
+// whether one is a NaN
+template <typename H>
+__device__ __noinline__ uint32_t finite8(uint4 raw, uint32_t most, bool* nan) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t u = (w[k / 2] >> (16 * (k & 1))) & 0x7fffu;
+    if (u > inf16<H>()) *nan = true;
+    if (u < inf16<H>() && u > most) most = u;
+  }
+  return most;
+}
+// eight values times f as codes (f a power of two: exact before the rounding,
+// but for what is far below the codes); a NaN is 0
+template <typename H, bool NANS>
+__device__ __forceinline__ uint2 code8(uint4 raw, float f) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float lo = value16<H>(w[k] & 0xffffu), hi = value16<H>(w[k] >> 16);
+    if (NANS) {
+      lo = lo == lo ? lo : 0.f;
+      hi = hi == hi ? hi : 0.f;
+    }
+    o[k] = to_e4m3x2(lo * f, hi * f);
+  }
+  return make_uint2(o[0] | o[1] << 16, o[2] | o[3] << 16);
+}
+
+// Few new tokens (a decoder step): a warp writes one page's of one head, keys
+// or values. Bound by the chain of reads that leads to the page.
+template <typename H>
+__global__ void __launch_bounds__(128) k_kv8_append_few(const Kv8AppendArgs a, int width, long long units) {
+  const long long unit = (long long)blockIdx.x * 4 + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
   pdl_wait();
   pdl_trigger();
   if (unit >= units) return;
@@ -70,78 +152,120 @@ __global__ void __launch_bounds__(128) k_kv8_append(const Kv8AppendArgs a, int w
   long long rest = unit / 2;
   const int h = (int)(rest % c.n_kv_heads);
   rest /= c.n_kv_heads;
-  const int w = (int)(rest % width), s = (int)(rest / width);
-  const int r0 = a.new_off[s], n = a.new_off[s + 1] - r0, len = a.lens[s];
-  if (n == 0) return;
-  if (r0 < 0 || n < 0 || n > a.max_new || r0 > a.rows - n || len < n || len > (long long)c.table_ld * c.page) {
-    if (lane == 0) report_error(a.err, DEV_ERR_BAD_SHAPE);
-    return;
-  }
-  const int base = len - n, pg = base / c.page + w;  // tokens before, this unit's page
-  if ((long long)pg * c.page >= len) return;
-  const int id = c.table[(long long)s * c.table_ld + pg];
-  if (id < 0 || id >= c.n_pages) {
-    if (lane == 0) report_error(a.err, DEV_ERR_BAD_SHAPE);
-    return;
-  }
-  const int t0 = max(base - pg * c.page, 0), t1 = min(len - pg * c.page, c.page);  // new tokens of the page
+  const PageShare p = page_share(a, (int)(rest / width), (int)(rest % width), lane == 0);
+  if (!p.on) return;
   const long long ld = x ? a.ldv : a.ldk;
-  const H* src = reinterpret_cast<const H*>(x ? a.v : a.k) + (long long)(r0 + pg * c.page + t0 - base) * ld + h * D;
-  const long long ph = (long long)id * c.n_kv_heads + h;
+  const H* src = reinterpret_cast<const H*>(x ? a.v : a.k) + p.row * ld + h * D;
+  const long long ph = (long long)p.id * c.n_kv_heads + h;
   uint8_t* dst = (x ? c.v : c.k) + ph * c.page * D;
   float* scale = (x ? c.v_scale : c.k_scale) + ph;
-
-  // ---- the largest new value
-  float most = 0.f;
-  bool nan = false;
-  for (int i = lane; i < (t1 - t0) * vec; i += T) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(src + (long long)(i / vec) * ld + i % vec * 8);
-    const H* y = reinterpret_cast<const H*>(&raw);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float f = fabsf(from_h(y[k]));
-      nan |= f != f;
-      if (f < INFINITY) most = fmaxf(most, f);
-    }
+  const int n_vec = (p.t1 - p.t0) * vec;
+  const int e0 = p.t0 > 0 ? exponent_of(*scale) : -127;
+  auto value = [&](int i) { return *reinterpret_cast<const uint4*>(src + (long long)(i / vec) * ld + i % vec * 8); };
+  uint32_t most = 0;
+  for (int i = lane; i < n_vec; i += 32) most = look8(value(i), most);
+  most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+  const bool special = most >= inf16<H>();
+  if (special) {
+    bool nan = false;
+    most = 0;
+    for (int i = lane; i < n_vec; i += 32) most = finite8<H>(value(i), most, &nan);
+    if (nan) report_error(a.err, DEV_ERR_NONFINITE);
+    most = __reduce_max_sync(0xffffffffu, most);
   }
-#pragma unroll
-  for (int k = 16; k > 0; k >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, k));
-  if constexpr (T > 32) {
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = most;
-    __syncthreads();
-    most = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-  }
-  if (nan) report_error(a.err, DEV_ERR_NONFINITE);
-  const int need = need_exp(most);
-  const int e0 = t0 > 0 ? exponent_of(*scale) : -127;
-  const int e = max(e0, need);
-  // ---- the page's older codes, where the scale grew
-  if (t0 > 0 && e > e0) {
+  const int e = max(e0, need_exp(value16<H>(most)));
+  if (p.t0 > 0 && e > e0) {  // the page's older codes, where the scale grew
     const float f = exp2i(e0 - e);
-    for (int i = lane; i < t0 * vec; i += T) {
-      uint2* p = reinterpret_cast<uint2*>(dst + i * 8);
-      *p = rescale8(*p, f);
+    for (int i = lane; i < p.t0 * vec; i += 32) {
+      uint2* q = reinterpret_cast<uint2*>(dst + i * 8);
+      *q = rescale8(*q, f);
     }
   }
-  // every lane has read the scale
-  if constexpr (T > 32)
-    __syncthreads();
-  else
-    __syncwarp();
+  __syncwarp();  // every lane has read the scale
   if (lane == 0) *scale = exp2i(e);
-  // ---- the new tokens
   const float f = exp2i(-e);
-  for (int i = lane; i < (t1 - t0) * vec; i += T) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(src + (long long)(i / vec) * ld + i % vec * 8);
-    const H* y = reinterpret_cast<const H*>(&raw);
-    float z[8];
+  for (int i = lane; i < n_vec; i += 32)
+    *reinterpret_cast<uint2*>(dst + (p.t0 * vec + i) * 8) = code8<H, true>(value(i), f);
+}
+
+// Many new tokens (a prompt): eight warps write one page's of eight heads (keys
+// and values counted apart), WPH warps a head where a head's page is more than
+// 4096 values. NV vectors of it stay in each lane's registers between the
+// search for the largest value and the rounding, so every value is read once,
+// and neighbouring heads of a row at the same time: a CTA for each head, whose
+// reads are 128 bytes apart from the next ones' by a whole row, reached half
+// the copy rate. 64 sequences of 1 to 1024 tokens, 8 heads of 64, pages of 64:
+// 24 us for 97 MB, 62% of the copy rate (41 us a CTA a head with two reads;
+// 47 us with maxima and checks in f32: the arithmetic on each value counts).
+template <typename H, int NV, int WPH>
+__global__ void __launch_bounds__(256, 3) k_kv8_append(const Kv8AppendArgs a, int width, int passes) {
+  __shared__ uint32_t s_max[2][8];
+  const Kv8& c = a.c;
+  const int D = c.head_dim, sh = D == 128 ? 4 : 3, vec = D / 8;
+  const int warp = threadIdx.x >> 5;
+  const int rest = blockIdx.x / passes;
+  const int unit = blockIdx.x % passes * (8 / WPH) + warp / WPH;  // 0 .. Hkv - 1 keys, then values
+  pdl_wait();
+  pdl_trigger();
+  const PageShare p = page_share(a, rest / width, rest % width, threadIdx.x == 0);
+  if (!p.on) return;
+  const bool have = unit < 2 * c.n_kv_heads;
+  const int x = have && unit >= c.n_kv_heads, h = have ? unit - x * c.n_kv_heads : 0;
+  const long long ld = x ? a.ldv : a.ldk;
+  const H* src = reinterpret_cast<const H*>(x ? a.v : a.k) + p.row * ld + h * D;
+  const long long ph = (long long)p.id * c.n_kv_heads + h;
+  uint8_t* dst = (x ? c.v : c.k) + ph * c.page * D;
+  float* scale = (x ? c.v_scale : c.k_scale) + ph;
+  const int n_vec = have ? (p.t1 - p.t0) * vec : 0;
+  const int lane = threadIdx.x % (32 * WPH);  // of the head's threads
+  uint4 raw[NV];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float v = from_h(y[k]);
-      z[k] = v == v ? v * f : 0.f;
+  for (int j = 0; j < NV; ++j) {
+    const int i = j * 32 * WPH + lane;
+    raw[j] = make_uint4(0, 0, 0, 0);
+    if (i < n_vec) raw[j] = *reinterpret_cast<const uint4*>(src + (long long)(i >> sh) * ld + (i & (vec - 1)) * 8);
+  }
+  const int e0 = p.t0 > 0 ? exponent_of(*scale) : -127;
+  // over the head's threads (which passes every thread's reading of the scale)
+  auto joined = [&](uint32_t most, int k) -> uint32_t {
+    most = __reduce_max_sync(0xffffffffu, most);
+    if constexpr (WPH > 1) {
+      if ((threadIdx.x & 31) == 0) s_max[k][warp] = most;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WPH; ++w) most = max(most, s_max[k][warp / WPH * WPH + w]);
     }
-    *reinterpret_cast<uint2*>(dst + (t0 * vec + i) * 8) =
-        make_uint2(to_e4m3x2(z[0], z[1]) | to_e4m3x2(z[2], z[3]) << 16, to_e4m3x2(z[4], z[5]) | to_e4m3x2(z[6], z[7]) << 16);
+    return most;
+  };
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) most = look8(raw[j], most);
+  most = joined(max(most & 0xffffu, most >> 16), 0);
+  const bool special = __syncthreads_or(most >= inf16<H>());
+  if (special) {
+    bool nan = false;
+    most = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) most = finite8<H>(raw[j], most, &nan);
+    if (nan) report_error(a.err, DEV_ERR_NONFINITE);
+    most = joined(most, 1);
+  }
+  if (!have) return;
+  const int e = max(e0, need_exp(value16<H>(most)));
+  if (p.t0 > 0 && e > e0) {  // the page's older codes, where the scale grew
+    const float f = exp2i(e0 - e);
+    for (int i = lane; i < p.t0 * vec; i += 32 * WPH) {
+      uint2* q = reinterpret_cast<uint2*>(dst + i * 8);
+      *q = rescale8(*q, f);
+    }
+  }
+  if (lane == 0) *scale = exp2i(e);
+  const float f = exp2i(-e);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int i = j * 32 * WPH + lane;
+    if (i < n_vec)
+      *reinterpret_cast<uint2*>(dst + (p.t0 * vec + i) * 8) = special ? code8<H, true>(raw[j], f) : code8<H, false>(raw[j], f);
   }
 }
 
@@ -226,8 +350,18 @@ cudaError_t append_h(const Kv8AppendArgs& a, cudaStream_t st) {
   const long long units = (long long)a.n_seqs * width * a.c.n_kv_heads * 2;
   if (units > 0x7fffffffLL) return cudaErrorInvalidValue;
   if (a.max_new <= 4)
-    return launch_pdl(k_kv8_append<H, 32>, dim3((unsigned)((units + 3) / 4)), dim3(128), 0, st, a, width, units);
-  return launch_pdl(k_kv8_append<H, 128>, dim3((unsigned)units), dim3(128), 0, st, a, width, units);
+    return launch_pdl(k_kv8_append_few<H>, dim3((unsigned)((units + 3) / 4)), dim3(128), 0, st, a, width, units);
+  auto many = [&](auto kern, int wph) {
+    const int passes = (2 * a.c.n_kv_heads * wph + 7) / 8;
+    return launch_pdl(kern, dim3((unsigned)((long long)a.n_seqs * width * passes)), dim3(256), 0, st, a, width, passes);
+  };
+  switch (a.c.page * a.c.head_dim / 1024) {
+    case 1: return many(k_kv8_append<H, 4, 1>, 1);
+    case 2: return many(k_kv8_append<H, 8, 1>, 1);
+    case 4: return many(k_kv8_append<H, 16, 1>, 1);
+    case 8: return many(k_kv8_append<H, 16, 2>, 2);
+    default: return many(k_kv8_append<H, 16, 4>, 4);
+  }
 }
 
 }  // namespace
