@@ -750,3 +750,240 @@ def test_kv8_reorder_refuses_on_the_device(cuda):
         assert torch.equal(c["table"][:2, 0].flip(0), table[:2, 0])  # the other item moved
         own = [p for p in table[2:].flatten().tolist() if 0 <= p < c["total"]]
         assert torch.equal(c["k"][own], pool[own])
+
+
+# ---------------------------------------------------------------- several at once, captured, other streams
+
+
+def test_small_workspaces_do_not_overlap(cuda):
+    """Two calls on two streams at once, each with its own workspace, give what
+    each gives alone."""
+    import pkc
+    import torch
+    H, D, t = 8, 64, 9000
+    g = torch.Generator().manual_seed(21)
+    args = []
+    for i in range(2):
+        q = torch.randn(1, H * D, generator=g).half().to(cuda)
+        kv = torch.randn(t, 2, H, D, generator=g).half().to(cuda)
+        n = pkc.cross_attention_workspace(1, 1, t, H, H, D)
+        assert n > 0  # the joined form
+        args.append(dict(q=q, kv=kv, ws=workspace(n, cuda), out=torch.zeros(1, H * D, dtype=torch.float16, device=cuda),
+                         q_off=offsets([1], cuda), kv_off=torch.zeros(1, dtype=torch.int32, device=cuda),
+                         kv_len=torch.full((1,), t, dtype=torch.int32, device=cuda)))
+
+    def call(a, out, st):
+        pkc.cross_attention(a["q"].data_ptr(), a["kv"].data_ptr(), a["kv"][:, 1].data_ptr(), a["q_off"].data_ptr(),
+                            a["kv_off"].data_ptr(), a["kv_len"].data_ptr(), 1, H, H, D, q_rows=1, kv_rows=t, max_q=1,
+                            max_kv=t, ldk=2 * H * D, ldv=2 * H * D, bf16=False, out=out.data_ptr(),
+                            workspace=a["ws"].data_ptr(), workspace_bytes=a["ws"].numel(), stream=st)
+
+    want = []
+    for a in args:
+        o = torch.zeros_like(a["out"])
+        call(a, o, stream())
+        torch.cuda.synchronize()
+        want.append(o)
+    s = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for a, st in zip(args, s):
+            call(a, a["out"], st.cuda_stream)
+    torch.cuda.synchronize()
+    for a, w in zip(args, want):
+        assert torch.equal(a["out"], w)
+
+
+class Decoder:
+    """A small attention decoder (random weights, 16-bit) run by the library's
+    operators: self attention over the 8-bit cache, cross attention to encoder
+    states, logits, selection, reordering."""
+
+    def __init__(self, cuda, B, K, page, steps, dt, *, layers=2, H=4, Hkv=2, D=64, V=211, seed=3):
+        import pkc
+        import torch
+        self.B, self.K, self.page, self.steps, self.L, self.H, self.Hkv, self.D, self.V = B, K, page, steps, layers, H, Hkv, D, V
+        self.dev, self.dt, self.eos = cuda, dt, 7
+        d = self.d = H * D
+        g = torch.Generator().manual_seed(seed)
+        mk = lambda *s, scale: (torch.randn(*s, generator=g) * scale).to(dt).to(cuda)  # noqa: E731
+        self.embed = mk(V, d, scale=1.0)
+        self.w = [dict(qkv=mk(d, d + 2 * Hkv * D, scale=d ** -0.5), o=mk(d, d, scale=d ** -0.5), cq=mk(d, d, scale=d ** -0.5),
+                       co=mk(d, d, scale=d ** -0.5)) for _ in range(layers)]
+        self.head = mk(d, V, scale=3 * d ** -0.5)
+        self.enc_len = [40, 3, 77, 0, 25][:B]
+        M = sum(self.enc_len)
+        self.enc = [mk(M, 2, H * D, scale=1.0) for _ in range(layers)]
+        self.kv_off = offsets(self.enc_len, cuda)[:-1].contiguous()
+        self.kv_len = torch.tensor(self.enc_len, dtype=torch.int32, device=cuda)
+        S = B * K
+        self.caches = [make_cache(cuda, S, [steps + 1] * S, Hkv, D, page, seed=i) for i in range(layers)]
+        self.one = offsets([1] * S, cuda)
+        self.beams = offsets([K] * B, cuda)
+        self.lens = torch.zeros(S, dtype=torch.int32, device=cuda)
+        self.token = torch.zeros(B, K, dtype=torch.int32, device=cuda)
+        self.parent = torch.zeros(B, K, dtype=torch.int32, device=cuda)
+        self.cum = torch.zeros(B, K, device=cuda)
+        self.cum[:, 1:] = float("-inf")
+        self.done = torch.zeros(B, K, dtype=torch.uint8, device=cuda)
+        self.history = torch.full((S, steps), -1, dtype=torch.int32, device=cuda)
+        self.step_at = torch.zeros(1, dtype=torch.int64, device=cuda)
+        self.seen = []
+        self.ws = workspace(max(pkc.cross_attention_workspace(B, K, 77, H, H, D), pkc.kv8_attention_workspace(
+            self.caches[0]["c"], S, 1, steps, H)), cuda)
+
+    def step(self):
+        import pkc
+        import torch
+        B, K, S, H, D, d = self.B, self.K, self.B * self.K, self.H, self.D, self.d
+        bf, st = self.dt == torch.bfloat16, stream()
+        self.seen = []
+        self.lens += 1
+        x = self.embed[self.token.flatten().long()].float()
+        for i, (w, c) in enumerate(zip(self.w, self.caches)):
+            qkv = torch.nn.functional.layer_norm(x, (d,)).to(self.dt) @ w["qkv"]
+            n = self.Hkv * D
+            ld = qkv.stride(0)
+            pkc.kv8_append(c["c"], qkv[:, d:].data_ptr(), qkv[:, d + n:].data_ptr(), self.one.data_ptr(), self.lens.data_ptr(), S,
+                           rows=S, max_new=1, ldk=ld, ldv=ld, bf16=bf, err=c["err"].data_ptr(), stream=st)
+            a = torch.empty(S, d, dtype=self.dt, device=self.dev)
+            pkc.kv8_attention(c["c"], qkv.data_ptr(), self.one.data_ptr(), self.lens.data_ptr(), S, H, q_rows=S, max_q=1,
+                              max_len=self.steps, ldq=ld, bf16=bf, out=a.data_ptr(), workspace=self.ws.data_ptr(),
+                              workspace_bytes=self.ws.numel(), err=c["err"].data_ptr(), stream=st)
+            x = x + (a @ w["o"]).float()
+            cq = torch.nn.functional.layer_norm(x, (d,)).to(self.dt) @ w["cq"]
+            ca = torch.empty(S, d, dtype=self.dt, device=self.dev)
+            e = self.enc[i]
+            pkc.cross_attention(cq.data_ptr(), e.data_ptr(), e[:, 1].data_ptr(), self.beams.data_ptr(), self.kv_off.data_ptr(),
+                                self.kv_len.data_ptr(), B, H, H, D, q_rows=S, kv_rows=e.shape[0], max_q=K, max_kv=77,
+                                ldk=2 * d, ldv=2 * d, bf16=bf, out=ca.data_ptr(), workspace=self.ws.data_ptr(),
+                                workspace_bytes=self.ws.numel(), err=c["err"].data_ptr(), stream=st)
+            self.seen += [qkv, a, cq, ca]
+            x = x + (ca @ w["co"]).float()
+        logits = torch.nn.functional.layer_norm(x, (d,)).to(self.dt).float() @ self.head.float()
+        self.seen += [logits, self.cum.clone(), self.done.clone()]
+        pkc.beam_select(logits.data_ptr(), self.cum.data_ptr(), self.done.data_ptr(), B, K, self.V, eos=self.eos,
+                        score=self.cum.data_ptr(), parent=self.parent.data_ptr(), token=self.token.data_ptr(),
+                        finished_out=self.done.data_ptr(), stream=st)
+        for c in self.caches:
+            pkc.kv8_reorder(c["c"], self.parent.data_ptr(), self.lens.data_ptr(), B, K, err=c["err"].data_ptr(), stream=st)
+        pkc.beam_reorder(self.history.data_ptr(), self.parent.data_ptr(), B, K, row_bytes=4 * self.steps, err=self.caches[0]["err"].data_ptr(),
+                         stream=st)
+        self.history.scatter_(1, self.step_at.expand(S, 1), self.token.view(S, 1))
+        self.step_at += 1
+        # (the operators are done with these when the stream is; keep them until then)
+        self.keep = (x, logits)
+
+
+@pytest.mark.parametrize("bf16,B,K,page,steps", [(False, 3, 4, 16, 37), (True, 4, 8, 32, 20), (False, 5, 1, 16, 18)])
+def test_decoder_beam_search(cuda, bf16, B, K, page, steps):
+    """A whole beam search: after every step each operator's output is checked
+    against the 64-bit restatement of the same step, whose caches and
+    hypotheses follow their own history (dense, copied at each reordering)."""
+    import decode_ref
+    import torch
+    dt = torch.bfloat16 if bf16 else torch.float16
+    m = Decoder(cuda, B, K, page, steps, dt)
+    S, H, Hkv, D, d = B * K, m.H, m.Hkv, m.D, m.d
+    # the restatement: for each layer and sequence a cache of its own with identity pages
+    n_pg = -(-(steps + 1) // page)
+    refs = [[decode_ref.RefCache(n_pg, Hkv, page, D) for _ in range(S)] for _ in range(m.L)]
+    texts = [[] for _ in range(S)]
+    for t in range(1, steps + 1):
+        m.step()
+        torch.cuda.synchronize()
+        assert all(int(c["err"]) == 0 for c in m.caches)
+        for i in range(m.L):
+            qkv, a, cq, ca = m.seen[4 * i: 4 * i + 4]
+            for s in range(S):
+                r = refs[i][s]
+                r.append(list(range(n_pg)), qkv[s, d:].double().view(1, 2, Hkv, D).cpu(), t)
+                k, v = (y.to(cuda) for y in r.dense(list(range(n_pg)), t))
+                o, A, S_ = decode_ref.attention(qkv[s, :d].double().view(1, H, D), k, v, D ** -0.5, True)
+                tol = decode_ref.attention_tolerance(o, A, S_, float(v.abs().max()), t, D, dt, torch.float16)
+                assert ((a[s].double().view(1, H, D) - o).abs() <= tol).all(), (t, i, s)
+            for b in range(B):
+                e = m.enc[i][int(m.kv_off[b]): int(m.kv_off[b]) + m.enc_len[b]].double().view(-1, 2, H, D)
+                o, A, S_ = decode_ref.attention(cq[b * K:(b + 1) * K].double().view(K, H, D), e[:, 0], e[:, 1], D ** -0.5, False)
+                v_max = float(e[:, 1].abs().max()) if m.enc_len[b] else 0.0
+                tol = decode_ref.attention_tolerance(o, A, S_, v_max, m.enc_len[b], D, dt, dt)
+                assert ((ca[b * K:(b + 1) * K].double().view(K, H, D) - o).abs() <= tol).all(), (t, i, b)
+        logits, cum, done = m.seen[-3:]
+        rs, rp, rt, rd = decode_ref.beam_select(logits.view(B, K, -1), cum, done.bool(), m.eos)
+        assert torch.equal(m.parent.long(), rp) and torch.equal(m.token.long(), rt) and torch.equal(m.done.bool(), rd)
+        src = [b * K + int(rp[b, k]) for b in range(B) for k in range(K)]
+        import copy
+        refs = [[copy.deepcopy(layer[j]) for j in src] for layer in refs]
+        texts = [texts[j] + [int(rt.flatten()[s])] for s, j in enumerate(src)]
+        assert m.history[:, :t].tolist() == texts
+    assert len({tuple(x) for x in texts}) > 1 or K == 1
+
+
+def test_decoder_step_captured_and_replayed(cuda):
+    """One captured step replayed (lengths, tokens and tables move on the
+    device) takes the path of the eager steps, bit for bit, also on another
+    stream."""
+    import torch
+    runs = []
+    for how in ("eager", "graph", "side"):
+        m = Decoder(cuda, 3, 4, 16, 24, torch.float16)
+        if how == "graph":
+            # (a warm-up step outside the capture, on a decoder of its own)
+            Decoder(cuda, 3, 4, 16, 24, torch.float16).step()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                m.step()
+            for _ in range(24):
+                g.replay()
+        elif how == "side":
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                for _ in range(24):
+                    m.step()
+        else:
+            for _ in range(24):
+                m.step()
+        torch.cuda.synchronize()
+        assert all(int(c["err"]) == 0 for c in m.caches)
+        runs.append(m)
+    for m in runs[1:]:
+        assert torch.equal(m.history, runs[0].history) and torch.equal(m.cum, runs[0].cum)
+        for c, e in zip(m.caches, runs[0].caches):
+            assert torch.equal(c["table"], e["table"]) and torch.equal(c["k"], e["k"]) and torch.equal(c["v"], e["v"])
+
+
+def test_a_prompt_then_steps_equals_one_pass(cuda):
+    """Appending and attending in chunks (the many-row form), then token by
+    token, gives the rows that one pass over all tokens gives, as near as the
+    page scales allow: the cache of a page that grew is rounded again, so the
+    pages here are filled with values of one size."""
+    import torch
+    H, Hkv, D, page, n = 4, 2, 64, 32, 300
+    g = torch.Generator().manual_seed(31)
+    sign = (torch.randint(0, 2, (n, 2, Hkv, D), generator=g) * 2 - 1).float()
+    new = sign * (1 + torch.randint(0, 8, (n, 2, Hkv, D), generator=g) / 8)
+    new[:, :, :, 0] = 1.875  # the largest, in every token: one scale, and every value an e4m3 value
+    new = new.half().to(cuda)
+    q = torch.randn(n, H * D, generator=g).half().to(cuda)
+    whole = make_cache(cuda, 1, [n], Hkv, D, page)
+    append(whole, new, [n], [n])
+    want = torch.zeros_like(q)
+    run_kv8(whole, q, [n], [n], H, want)
+    parts = make_cache(cuda, 1, [n], Hkv, D, page, seed=5)
+    out = torch.zeros_like(q)
+    at = 0
+    for size in (150, 3, 1, 1, 60, 20, 1, 64):
+        append(parts, new[at:at + size], [size], [at + size])
+        o = torch.zeros_like(q[at:at + size])
+        run_kv8(parts, q[at:at + size].contiguous(), [size], [at + size], H, o)
+        out[at:at + size] = o
+        at += size
+    assert at == n
+    # the same sums in another order: f16 probabilities, one rounding of the output
+    assert ((out.double() - want.double()).abs() <= 2 * (2.0 ** -11 + 2.0 ** -11) * 1.875).all()
+
+
+def test_negative_and_zero_scale(cuda):
+    """scale may be negative or zero (even weights)."""
+    for scale in (-0.2, 0.0):
+        check_cross(cuda, [3, 140], [50, 90], 4, 2, 64, False, scale=scale)
