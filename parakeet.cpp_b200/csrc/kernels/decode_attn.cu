@@ -706,7 +706,7 @@ struct Plan {
   bool clustered;                       // the parts are joined in a cluster
   long long blocks;
 };
-Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, bool tiles = true) {
+Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, bool q8, bool tiles = true) {
   Plan p;
   const long long rows = (long long)max_q * (n_heads / n_kv_heads);
   if (rows > kFewRows && tiles) {
@@ -716,8 +716,10 @@ Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, 
     p.warps = 0;
     p.clustered = false;
     // parts of at least 512 keys (a part costs as much as six more tiles),
-    // until two CTAs run on every SM
-    const long long want = (2LL * kSms + p.blocks - 1) / (p.blocks > 0 ? p.blocks : 1), most = max_kv / 512;
+    // until two CTAs run on every SM; twice as many over the 8-bit cache, whose
+    // tiles cost more, so that uneven lengths count more
+    const long long fill = (q8 ? 4LL : 2LL) * kSms;
+    const long long want = (fill + p.blocks - 1) / (p.blocks > 0 ? p.blocks : 1), most = max_kv / 512;
     const long long n = want < most ? want : most;
     p.n_split = n < 1 ? 1 : n > 64 ? 64 : (int)n;
     return p;
@@ -773,7 +775,7 @@ cudaError_t launch_w(const DecodeAttnArgs& a, const Plan& p, cudaStream_t st) {
 
 template <typename H, bool Q8, int D, int WT>
 cudaError_t launch_rows(const DecodeAttnArgs& a, cudaStream_t st) {
-  const Plan p = plan_rows(a.n_items, a.max_q, a.max_kv, a.n_heads, a.n_kv_heads, attn_tiles_fit(a));
+  const Plan p = plan_rows(a.n_items, a.max_q, a.max_kv, a.n_heads, a.n_kv_heads, Q8, attn_tiles_fit(a));
   if (p.blocks * p.n_split * p.rows > 0x7fffffffLL) return cudaErrorInvalidValue;
   if (p.warps == 0) {
     const cudaError_t e = attn_tiles_launch(a, is_bf16<H>::value, p.row_tiles, p.n_split, st);
@@ -798,8 +800,8 @@ cudaError_t launch_h(const DecodeAttnArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-size_t decode_attn_ws_bytes(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, int head_dim, bool) {
-  const Plan p = plan_rows(n_items, max_q, max_kv, n_heads, n_kv_heads);
+size_t decode_attn_ws_bytes(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, int head_dim, bool q8) {
+  const Plan p = plan_rows(n_items, max_q, max_kv, n_heads, n_kv_heads, q8);
   return p.n_split == 1 || p.clustered ? 0 : (size_t)p.blocks * p.n_split * p.rows * (head_dim + 2) * sizeof(float);
 }
 

@@ -259,7 +259,8 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
         }
         const uint64_t dv = smem_desc_sw128_mn(ring_addr(n), KN * 128, 1024);
         const uint32_t pa = tmem + 64u * (uint32_t)buf;
-        const int parts = Q8 ? info(t)->parts : 1, steps = KN / 16 / parts;
+        const int parts = Q8 ? info(t)->parts : 1;
+        const int part_shift = parts == 1 ? 2 : parts == 2 ? 1 : 0;  // of 16-key steps
         for (int j = 0; j < parts && ok; ++j) {
           ok = wwait(B_PFULL + buf, (pf >> buf) & 1u);
           pf ^= 1u << buf;
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < KN / 16; ++kk)
-            if (kk / steps == j)
+            if (kk >> part_shift == j)
               umma_f16_ts_if(leader, tmem + TM_O, pa + 8u * kk, dv + (uint64_t)((kk * 16 * 128) >> 4), id_pv,
                              (t > 0 || kk > 0) ? 1u : 0u);
           if (j == parts - 1) umma_commit_if(leader, bar(B_REMPTY + n % RING));
