@@ -165,16 +165,31 @@ __global__ void __launch_bounds__(32 * W, NB == 1 ? 12 / W : 8 / W) k_attn_rows(
   const int cnt = t0 < t_end ? (t_end - t0 + W - 1) / W : 0;
   uint8_t* ring = smem + warp * L::kWarp;
   const uint32_t ring_s = smem_u32(ring);
-  const uint8_t* kbase = nullptr;
-  const uint8_t* vbase = nullptr;
-  if constexpr (!Q8) {
-    kbase = reinterpret_cast<const uint8_t*>(reinterpret_cast<const H*>(a.k) + (long long)it.kv0 * a.ldk + h * D);
-    vbase = reinterpret_cast<const uint8_t*>(reinterpret_cast<const H*>(a.v) + (long long)it.kv0 * a.ldv + h * D);
+  // this lane's 16 bytes of a tile: chunk `ch` of rows r0, r0 + RS, ...
+  constexpr int RS = 512 / RB;
+  const int r0 = lane / (RB / 16), ch = lane % (RB / 16);
+  const uint32_t kd0 = key_at<RB>(r0, ch), vd0 = L::kTile + value_at<RB>(r0, ch);
+  const uint8_t *lane_k, *lane_v;  // 8-bit: of page 0 of this head; else of the item's first row
+  long long k_row = RB, v_row = RB;
+  int shift = 0;  // of a page in tokens
+  const int* table = nullptr;
+  long long page_bytes = 0;
+  if constexpr (Q8) {
+    const Kv8& cc = a.cache;
+    shift = __ffs(cc.page) - 1;
+    table = cc.table + (long long)b * cc.table_ld;
+    page_bytes = ((long long)cc.n_kv_heads << shift) * D;
+    lane_k = cc.k + ((long long)h << shift) * D + lane * 16;
+    lane_v = cc.v + ((long long)h << shift) * D + lane * 16;
+  } else {
+    k_row = a.ldk * 2;
+    v_row = a.ldv * 2;
+    lane_k = reinterpret_cast<const uint8_t*>(reinterpret_cast<const H*>(a.k) + (long long)(it.kv0 + r0) * a.ldk + h * D) + ch * 16;
+    lane_v = reinterpret_cast<const uint8_t*>(reinterpret_cast<const H*>(a.v) + (long long)(it.kv0 + r0) * a.ldv + h * D) + ch * 16;
   }
   auto page_of = [&](int i) -> int {  // page of the warp's i-th tile
     if constexpr (!Q8) return 0;
-    if (i >= cnt) return 0;
-    return a.cache.table[(long long)b * a.cache.table_ld + (t0 + W * i) * WT / a.cache.page];
+    return i < cnt ? table[((t0 + W * i) * WT) >> shift] : 0;
   };
   // copy the warp's i-th tile; rows that no query row sees become zeros (a NaN
   // there would survive a probability of zero)
@@ -182,46 +197,41 @@ __global__ void __launch_bounds__(32 * W, NB == 1 ? 12 / W : 8 / W) k_attn_rows(
     if (i < cnt) {
       const int k0 = (t0 + W * i) * WT, left = vmax - k0;
       const uint32_t dst = ring_s + (i % kStages) * L::kStage;
-      const uint8_t *kp = kbase, *vp = vbase;
-      long long kst = RB, vst = RB;
+      const uint8_t *kp, *vp;
       bool on = true;
       if constexpr (Q8) {
         const Kv8& cc = a.cache;
-        on = id >= 0 && id < cc.n_pages;
-        const long long ph = (long long)(on ? id : 0) * cc.n_kv_heads + h;
-        kp = cc.k + (ph * cc.page + k0 % cc.page) * D;
-        vp = cc.v + (ph * cc.page + k0 % cc.page) * D;
-        const uint32_t sc = ring_s + kStages * L::kStage + (i % kStages) * 16;
+        on = (unsigned)id < (unsigned)cc.n_pages;
+        const long long at = (long long)(on ? id : 0) * page_bytes + (k0 & (cc.page - 1)) * D;
+        kp = lane_k + at;
+        vp = lane_v + at;
+        const uint32_t sc = kStages * L::kStage + (i % kStages) * 16;
         if (on) {
-          if (lane < 2) cp_async4(sc + 4 * lane, (lane ? cc.v_scale : cc.k_scale) + ph);
+          if (lane < 2) cp_async4(ring_s + sc + 4 * lane, (lane ? cc.v_scale : cc.k_scale) + (long long)id * cc.n_kv_heads + h);
         } else if (lane == 0) {
           // the keys of a page that is none are not seen
           report_error(a.err, DEV_ERR_BAD_SHAPE);
-          *reinterpret_cast<float*>(ring + kStages * L::kStage + (i % kStages) * 16) = -1.f;
+          *reinterpret_cast<float*>(ring + sc) = -1.f;
         }
       } else {
-        kst = a.ldk * 2;
-        vst = a.ldv * 2;
-        kp += k0 * kst;
-        vp += k0 * vst;
+        kp = lane_k + k0 * k_row;
+        vp = lane_v + k0 * v_row;
       }
-// a lane copies chunk `ch` of rows r0, r0 + 512 / RB, ...
-      constexpr int RS = 512 / RB;
-      const int r0 = lane / (RB / 16), ch = lane % (RB / 16);
-      kp += r0 * kst + ch * 16;
-      vp += r0 * vst + ch * 16;
+      // (the permutation of a value row's chunks changes with j alone)
+      constexpr int VX = RB == 64 ? 0 : RB == 128 ? 4 : 6;
       if (left >= WT && on) {
 #pragma unroll
-        for (int j = 0; j < WT / RS; ++j) cp_async16(dst + key_at<RB>(r0 + j * RS, ch), kp + j * RS * kst, 16);
+        for (int j = 0; j < WT / RS; ++j) cp_async16(dst + kd0 + j * 512, kp + (Q8 ? j * 512 : j * RS * k_row), 16);
 #pragma unroll
         for (int j = 0; j < WT / RS; ++j)
-          cp_async16(dst + L::kTile + value_at<RB>(r0 + j * RS, ch), vp + j * RS * vst, 16);
+          cp_async16(dst + (vd0 ^ (((j * RS) & VX) * 16)) + j * 512, vp + (Q8 ? j * 512 : j * RS * v_row), 16);
       } else {
 #pragma unroll
         for (int j = 0; j < WT / RS; ++j) {
-          const bool in = on && r0 + j * RS < left;
-          cp_async16(dst + key_at<RB>(r0 + j * RS, ch), in ? kp + j * RS * kst : kp - r0 * kst, in ? 16 : 0);
-          cp_async16(dst + L::kTile + value_at<RB>(r0 + j * RS, ch), in ? vp + j * RS * vst : vp - r0 * vst, in ? 16 : 0);
+          const bool in = on && r0 + j * RS < left;  // (rows that are not read start nowhere else than the item's first)
+          cp_async16(dst + kd0 + j * 512, in ? kp + j * RS * k_row : lane_k - (Q8 ? 0 : r0 * k_row), in ? 16 : 0);
+          cp_async16(dst + (vd0 ^ (((j * RS) & VX) * 16)) + j * 512, in ? vp + j * RS * v_row : lane_v - (Q8 ? 0 : r0 * v_row),
+                     in ? 16 : 0);
         }
       }
     }
