@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/pkc.h"
@@ -32,8 +33,12 @@ pkc_status bad(const char* what, const char* why) {
 
 bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// The stream and the given memory belong to the current device.
-pkc_status check_device(const char* what, void* stream, const void* const* ptrs, int n) {
+// The stream and the given memory belong to the current device; arrays of
+// 32-bit numbers are aligned. NULLs are passed over.
+pkc_status check_device(const char* what, void* stream, std::initializer_list<const void*> ints,
+                        std::initializer_list<const void*> more) {
+  for (const void* p : ints)
+    if (!aligned(p, 4)) return bad(what, "an array of 32-bit numbers is not aligned");
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) {
@@ -55,15 +60,17 @@ pkc_status check_device(const char* what, void* stream, const void* const* ptrs,
     }
     if (sdev != dev) return bad(what, "the stream belongs to another device than the current one");
   }
-  for (int i = 0; i < n; ++i) {
-    cudaPointerAttributes at;
-    if (cudaPointerGetAttributes(&at, ptrs[i]) != cudaSuccess) {
-      cudaGetLastError();
-      return bad(what, "a pointer is not device memory");
+  for (const auto* list : {&ints, &more})
+    for (const void* p : *list) {
+      if (!p) continue;
+      cudaPointerAttributes at;
+      if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        cudaGetLastError();
+        return bad(what, "a pointer is not device memory");
+      }
+      if (at.type != cudaMemoryTypeManaged && (at.type != cudaMemoryTypeDevice || at.device != dev))
+        return bad(what, "memory of the host or of another device than the current one");
     }
-    if (at.type != cudaMemoryTypeManaged && (at.type != cudaMemoryTypeDevice || at.device != dev))
-      return bad(what, "memory of the host or of another device than the current one");
-  }
   return PKC_OK;
 }
 
@@ -130,8 +137,9 @@ extern "C" pkc_status pkc_cross_attention(const void* q, long long ldq, const in
     const size_t need = pkc::decode_attn_ws_bytes(B, max_q, max_kv, n_heads, n_kv_heads, head_dim, false);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
       return bad(what, "the workspace is missing, too small or not 16-byte aligned");
-    const void* ptrs[3] = {q, out, k};
-    const pkc_status ds = check_device(what, stream, ptrs, kv_rows > 0 ? 3 : 2);
+    const pkc_status ds = check_device(what, stream, {q_off, kv_off, kv_len, err},
+                                       {q, out, kv_rows > 0 ? k : nullptr, kv_rows > 0 ? v : nullptr,
+                                        need > 0 ? workspace : nullptr});
     if (ds != PKC_OK) return ds;
     pkc::DecodeAttnArgs a{};
     a.q = q; a.ldq = ldq; a.q_off = q_off; a.max_q = max_q; a.q_rows = q_rows;
@@ -158,8 +166,8 @@ extern "C" pkc_status pkc_kv8_append(const pkc_kv8_cache* cache, const void* k, 
     const char* why = rows_fault(k, ldk, row, "k rows must be 16-byte aligned and not overlap");
     if (!why) why = rows_fault(v, ldv, row, "v rows must be 16-byte aligned and not overlap");
     if (why) return bad(what, why);
-    const void* ptrs[2] = {k, cache->k};
-    const pkc_status ds = check_device(what, stream, ptrs, 2);
+    const pkc_status ds = check_device(what, stream, {new_off, lens, cache->table, cache->k_scale, cache->v_scale, err},
+                                       {k, v, cache->k, cache->v});
     if (ds != PKC_OK) return ds;
     pkc::Kv8AppendArgs a{kv8_of(cache), k, v, ldk, ldv, new_off, lens, n_seqs, rows, max_new, err};
     return launched(what, pkc::kv8_append_launch(a, dtype == 1, reinterpret_cast<cudaStream_t>(stream)));
@@ -196,8 +204,8 @@ extern "C" pkc_status pkc_kv8_attention(const pkc_kv8_cache* cache, const void* 
         pkc::decode_attn_ws_bytes(n_seqs, max_q, max_len, n_heads, cache->n_kv_heads, cache->head_dim, true);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
       return bad(what, "the workspace is missing, too small or not 16-byte aligned");
-    const void* ptrs[3] = {q, out, cache->k};
-    const pkc_status ds = check_device(what, stream, ptrs, 3);
+    const pkc_status ds = check_device(what, stream, {q_off, lens, cache->table, cache->k_scale, cache->v_scale, err},
+                                       {q, out, cache->k, cache->v, need > 0 ? workspace : nullptr});
     if (ds != PKC_OK) return ds;
     pkc::DecodeAttnArgs a{};
     a.q = q; a.ldq = ldq; a.q_off = q_off; a.max_q = max_q; a.q_rows = q_rows;
@@ -218,8 +226,8 @@ extern "C" pkc_status pkc_kv8_reorder(const pkc_kv8_cache* cache, const int* par
       return bad(what, "B must be in [0, 65535] and K in [1, 32]");
     if (B == 0) return PKC_OK;
     if (!parent || !lens) return bad(what, "a pointer is NULL");
-    const void* ptrs[2] = {parent, cache->k};
-    const pkc_status ds = check_device(what, stream, ptrs, 2);
+    const pkc_status ds = check_device(what, stream, {parent, lens, cache->table, cache->k_scale, cache->v_scale, err},
+                                       {cache->k, cache->v});
     if (ds != PKC_OK) return ds;
     return launched(what, pkc::kv8_reorder_launch(kv8_of(cache), parent, lens, B, K, err,
                                                   reinterpret_cast<cudaStream_t>(stream)));
@@ -237,11 +245,8 @@ extern "C" pkc_status pkc_beam_select(const void* logits, long long ld, int dtyp
     if (dtype < 0 || dtype > 2) return bad(what, "dtype must be 0 (f16), 1 (bf16) or 2 (f32)");
     if (B == 0) return PKC_OK;
     if (!logits || !cum || !score || !parent || !token) return bad(what, "a pointer is NULL");
-    if (!aligned(logits, dtype == 2 ? 4 : 2) || !aligned(cum, 4) || !aligned(score, 4) || !aligned(parent, 4) ||
-        !aligned(token, 4))
-      return bad(what, "a pointer is not aligned to its type");
-    const void* ptrs[2] = {logits, score};
-    const pkc_status ds = check_device(what, stream, ptrs, 2);
+    if (!aligned(logits, dtype == 2 ? 4 : 2)) return bad(what, "logits are not aligned to their type");
+    const pkc_status ds = check_device(what, stream, {cum, score, parent, token}, {logits, finished, finished_out});
     if (ds != PKC_OK) return ds;
     pkc::BeamSelectArgs a{logits, ld, cum, finished, B, K, V, eos, score, parent, token, finished_out};
     return launched(what, pkc::beam_select_launch(a, dtype, reinterpret_cast<cudaStream_t>(stream)));
@@ -261,8 +266,7 @@ extern "C" pkc_status pkc_beam_reorder(void* state, const int* parent, int B, in
       return bad(what, "blocks overlap: outer_stride is less than B * K * row_stride");
     if (B == 0 || n_outer == 0 || row_bytes == 0) return PKC_OK;
     if (!state || !parent) return bad(what, "a pointer is NULL");
-    const void* ptrs[2] = {state, parent};
-    const pkc_status ds = check_device(what, stream, ptrs, 2);
+    const pkc_status ds = check_device(what, stream, {parent, lens, err}, {state});
     if (ds != PKC_OK) return ds;
     pkc::BeamReorderArgs a{static_cast<uint8_t*>(state), parent, B, K, n_outer, n_outer > 1 ? outer_stride : 0,
                            row_stride, row_bytes, lens, lens ? unit_bytes : 0, err};

@@ -36,6 +36,7 @@ def cross(**kw):
     dict(head_dim=80), dict(head_dim=0), dict(n_heads=0), dict(n_kv_heads=0), dict(n_heads=3), dict(n_kv_heads=-2, n_heads=4),
     dict(q=P + 2), dict(out=P + 8), dict(k=P + 4), dict(v=P + 4), dict(ldq=255), dict(ldq=257), dict(ldk=120), dict(ldv=132),
     dict(ldo=0), dict(ldq=-256), dict(scale=float("nan")), dict(scale=float("inf")),
+    dict(q_off=P + 2), dict(kv_off=P + 1), dict(kv_len=P + 3), dict(err=P + 2),
 ])
 def test_cross_attention_refuses(kw):
     refused(cross, **kw)
@@ -43,9 +44,9 @@ def test_cross_attention_refuses(kw):
 
 def test_cross_attention_workspace_is_checked():
     import pkc
-    need = pkc.cross_attention_workspace(1, 1, 5000, 4, 2, 64)
+    need = pkc.cross_attention_workspace(1, 1, 20000, 4, 2, 64)
     assert need > 0
-    big = dict(max_q=1, max_kv=5000, kv_rows=5000)
+    big = dict(max_q=1, max_kv=20000, kv_rows=20000)
     assert "workspace" in refused(cross, workspace=0, **big)
     assert "workspace" in refused(cross, workspace_bytes=need - 1, **big)
     assert "workspace" in refused(cross, workspace=P + 4, **big)
@@ -74,7 +75,7 @@ def test_kv8_append_refuses():
         pkc.kv8_append(cache(), k, v, off, lens, n, rows=rows, max_new=max_new, bf16=False, **kw)
 
     for kw in (dict(k=0), dict(v=0), dict(off=0), dict(lens=0), dict(n=-1), dict(rows=-1), dict(max_new=-1), dict(k=P + 2),
-               dict(ldk=64), dict(ldv=132), dict(ldk=-128)):
+               dict(ldk=64), dict(ldv=132), dict(ldk=-128), dict(off=P + 2), dict(lens=P + 1), dict(err=P + 2)):
         refused(call, **kw)
     L = pkc.lib()
     assert L.pkc_kv8_append(None, P, 128, P, 128, P, P, 1, 1, 1, 0, None, None) == pkc.PKC_ERR_ARG
@@ -96,7 +97,7 @@ def test_kv8_attention_refuses():
 
 def test_kv8_reorder_refuses():
     import pkc
-    for args in ((0, P, 1, 2), (P, 0, 1, 2), (P, P, -1, 2), (P, P, 70000, 2), (P, P, 1, 0), (P, P, 1, 33)):
+    for args in ((0, P, 1, 2), (P, 0, 1, 2), (P, P, -1, 2), (P, P, 70000, 2), (P, P, 1, 0), (P, P, 1, 33), (P + 2, P, 1, 2), (P, P + 1, 1, 2)):
         refused(pkc.kv8_reorder, cache(), *args)
 
 
@@ -121,7 +122,7 @@ def test_beam_reorder_refuses():
 
     for kw in (dict(state=0), dict(parent=0), dict(B=-1), dict(B=70000), dict(K=0), dict(K=33), dict(row_bytes=-1),
                dict(row_stride=63), dict(n_outer=-1), dict(n_outer=70000), dict(n_outer=2, outer_stride=127),
-               dict(lens=P, unit_bytes=-1)):
+               dict(lens=P, unit_bytes=-1), dict(parent=P + 2), dict(lens=P + 1, unit_bytes=4)):
         refused(call, **kw)
 
 

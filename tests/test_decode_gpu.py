@@ -98,6 +98,12 @@ CROSS = [
     ([200, 130, 7], [437, 128, 513], 4, 4, 128),
     ([129, 257], [64, 191], 8, 2, 64),
     ([300], [1500], 6, 3, 64),
+    # heads that share a key head in odd numbers, and many of them
+    ([1, 2], [70, 33], 3, 1, 128),
+    ([60, 7], [100, 65], 6, 2, 64),
+    ([40, 1, 30], [129, 20, 64], 5, 1, 128),
+    ([1, 3], [300, 50], 24, 1, 64),
+    ([9, 20], [77, 210], 24, 1, 128),
 ]
 
 
@@ -155,6 +161,38 @@ def test_cross_attention_nan_stays_in_its_item(cuda, n):
     assert torch.isinf(out[n:2 * n, D + 5]).all()
     keep = [c for c in range(D, 2 * D) if c != D + 5]
     assert torch.equal(out[n:2 * n][:, keep], want[n:2 * n][:, keep])
+
+
+@pytest.mark.parametrize("n", [3, 140])
+def test_cross_attention_without_any_keys(cuda, n):
+    """kv_rows = 0 and no key memory at all: zeros."""
+    import pkc
+    import torch
+    q = torch.randn(n, 128, generator=torch.Generator().manual_seed(1)).half().to(cuda)
+    out = torch.full_like(q, -7.0)
+    z = torch.zeros(2, dtype=torch.int32, device=cuda)
+    qo = offsets([n - 1, 1], cuda)
+    pkc.cross_attention(q.data_ptr(), 0, 0, qo.data_ptr(), z.data_ptr(), z.data_ptr(), 2, 2, 2, 64, q_rows=n, kv_rows=0,
+                        max_q=n, max_kv=0, bf16=False, out=out.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("n", [2, 150])
+def test_cross_attention_beyond_32_bits(cuda, n):
+    """Keys whose rows lie behind the 2^32nd byte of their memory."""
+    import torch
+    D, t, ld = 64, 90, 65536
+    rows = (1 << 32) // (2 * ld) + t + 10
+    big = torch.empty(rows, ld, dtype=torch.float16, device=cuda)
+    g = torch.Generator().manual_seed(14)
+    kv = torch.randn(t, 2, 1, D, generator=g).half().to(cuda)
+    big[-t:, :2 * D] = kv.view(t, 2 * D)
+    q = torch.randn(n, D, generator=g).half().to(cuda)
+    want, out = torch.zeros_like(q), torch.zeros_like(q)
+    run_cross(cuda, q, kv, [n], [0], [t], 1, 1, D, want)
+    run_cross(cuda, q, big.as_strided((rows, 2, 1, D), (ld, D, D, 1)), [n], [rows - t], [t], 1, 1, D, out)
+    assert torch.equal(out, want) and float(out.abs().max()) > 0
 
 
 @pytest.mark.parametrize("n", [4, 140])
@@ -417,6 +455,9 @@ KV8 = [
     ([130, 9, 257], [130, 500, 700], 4, 4, 64, 64),
     ([200, 129], [513, 129], 8, 2, 128, 128),
     ([140, 33], [400, 47], 4, 1, 128, 32),
+    ([1, 3], [90, 40], 12, 1, 128, 16),
+    ([50, 11], [95, 60], 7, 1, 64, 32),
+    ([70], [333], 6, 2, 128, 128),
 ]
 
 
@@ -950,6 +991,59 @@ def test_decoder_step_captured_and_replayed(cuda):
         assert torch.equal(m.history, runs[0].history) and torch.equal(m.cum, runs[0].cum)
         for c, e in zip(m.caches, runs[0].caches):
             assert torch.equal(c["table"], e["table"]) and torch.equal(c["k"], e["k"]) and torch.equal(c["v"], e["v"])
+
+
+def test_the_first_call_may_be_captured(cuda):
+    """In a new process: the first call of every operator under capture, then
+    replayed."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch
+import test_decode_gpu as T
+dev = torch.device("cuda:0")
+m, e = (T.Decoder(dev, 2, 3, 16, 6, torch.bfloat16, seed=9) for _ in range(2))
+many = T.make_cache(dev, 1, [200], 2, 64, 32)
+kv = torch.randn(200, 2, 2, 64, device=dev).half()
+out = torch.zeros(200, 128, dtype=torch.float16, device=dev)
+no, ln = T.offsets([200], dev), torch.full((1,), 200, dtype=torch.int32, device=dev)
+zero = torch.zeros(1, dtype=torch.int32, device=dev)
+import pkc
+ws = T.workspace(max(1, pkc.kv8_attention_workspace(many["c"], 1, 200, 200, 2), pkc.cross_attention_workspace(1, 200, 200, 2, 2, 64)), dev)
+torch.zeros(8, 8, device=dev).half() @ torch.zeros(8, 8, device=dev).half()  # torch's own product needs a first call
+torch.zeros(8, 8, device=dev) @ torch.zeros(8, 8, device=dev)
+torch.zeros(8, 8, device=dev).bfloat16() @ torch.zeros(8, 8, device=dev).bfloat16()
+def prompt(st):
+    pkc.kv8_append(many["c"], kv.data_ptr(), kv[:, 1].data_ptr(), no.data_ptr(), ln.data_ptr(), 1, rows=200, max_new=200,
+                   ldk=256, ldv=256, bf16=False, err=many["err"].data_ptr(), stream=st)
+    pkc.kv8_attention(many["c"], kv.data_ptr(), no.data_ptr(), ln.data_ptr(), 1, 2, q_rows=200, max_q=200, max_len=200,
+                      ldq=256, bf16=False, out=out.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=ws.numel(),
+                      err=many["err"].data_ptr(), stream=st)
+    pkc.cross_attention(out.data_ptr(), kv.data_ptr(), kv[:, 1].data_ptr(), no.data_ptr(), zero.data_ptr(), ln.data_ptr(), 1, 2, 2, 64,
+                        q_rows=200, kv_rows=200, max_q=200, max_kv=200, ldk=256, ldv=256, bf16=False, out=res.data_ptr(),
+                        workspace=ws.data_ptr(), workspace_bytes=ws.numel(), err=many["err"].data_ptr(), stream=st)
+res = torch.zeros_like(out)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    m.step()
+    prompt(T.stream())
+for _ in range(6):
+    g.replay()
+torch.cuda.synchronize()
+a = res.clone()
+for _ in range(6):
+    e.step()
+prompt(T.stream())
+torch.cuda.synchronize()
+assert int(many["err"]) == 0 and torch.equal(a, res) and float(a.abs().max()) > 0
+assert torch.equal(m.history, e.history) and torch.equal(m.cum, e.cum)
+print("captured ok")
+""" % (os.path.dirname(os.path.abspath(__file__)), os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "parakeet.cpp_b200", "python"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured ok" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
 
 
 def test_a_prompt_then_steps_equals_one_pass(cuda):
