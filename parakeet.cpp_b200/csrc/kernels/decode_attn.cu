@@ -15,8 +15,8 @@
 // The products are taken transposed, S^T = K Q^T and O^T = V^T P^T: keys and
 // then output columns fill the 16 rows of mma.m16n8k16 and the few query rows
 // its 8 columns, so eight rows cost half of what 16 do (rows as the 16-row
-// side: 850 instructions a tile of 32 keys instead of about 400, and twice the
-// accumulators). P^T goes from the accumulator's layout to the operand's by
+// side: 850 instructions a tile of 32 keys of 128 8-bit columns instead of 510,
+// and twice the accumulators). P^T goes from the accumulator's layout to the operand's by
 // movmatrix.
 //
 // Fragments are 16-byte reads of the tile as it lies in memory: the order of
@@ -36,6 +36,13 @@
 // probabilities and take a product of their own, scaled in f32. bf16 queries
 // are brought to f16 with a power of two for each row (their 8 bits fit f16's
 // 11), which the softmax's factor takes back.
+//
+// Measured (copy rate 6539 GB/s): 512 sequences of 1 to 448 tokens, 8 heads of
+// 128, pages of 32: 46 us for 230 MB, 77% of it; 8 sequences of 9001 to 131071
+// tokens, 2 key heads for 16: 57 us for 265 MB, 71%; cross attention of 64 x 8
+// rows over 25 to 437 frames, 8 heads of 128: 17 us for 70 MB, 63%; one row
+// over 437 frames: 4.8 us. What is left is latency: the chain item -> table ->
+// codes at the start of each block of rows, and 40% of the issue slots.
 #include "common.cuh"
 #include "decode.h"
 #include "decode_common.cuh"
@@ -112,9 +119,9 @@ __device__ __forceinline__ int value_at(int r, int ch) {
 // the join of the warps reuses the rings.
 //
 // Two tiles a ring and 168 registers let twelve warps run on an SM, which is
-// what hides the latencies here (three tiles and eight warps: long contexts 68
-// instead of XX us); with two blocks of rows the registers leave eight, and
-// three tiles.
+// what hides the latencies here (against three tiles and eight warps: a step of
+// 512 short sequences 49 instead of 53 us, 8 long ones 60 instead of 68 us);
+// with two blocks of rows the registers leave eight, and three tiles.
 template <int RB, int WT, int NB>
 struct RowsLayout {
   static constexpr int kStages = NB == 1 ? 2 : 3;

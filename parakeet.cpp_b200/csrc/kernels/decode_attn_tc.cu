@@ -21,7 +21,7 @@
 // others: their scores are masked, and their values, which a zero probability
 // would not silence if they are not numbers, are zeroed in the last tile.
 //
-// The 8-bit cache's codes are turned into f16 by two warps that write the same
+// The 8-bit cache's codes are turned into f16 by four warps that write the same
 // ring: exactly, with the value scale taken in as a power of two relative to a
 // reference 2^ref in which O is kept. f16 holds e4m3 codes times 2^-15 .. 2^7
 // exactly, so ref stands while the pages stay in that range of it; else it
@@ -54,10 +54,11 @@ enum : int {
 
 // What the converting warps tell the softmax about a tile.
 struct TileInfo {
-  float ks[4];    // key scale of each 16 keys; -1: a page that is none
-  float grow[4];  // O is multiplied by this before part j of the tile is added
-  float ref;      // exponent that O is kept under, behind the tile
-  int parts;      // 1, or the tile's pages
+  float4 head;    // key scale (of a tile in one page; negative: a page that is none), what O is multiplied by
+                  // before the tile is added, the exponent that O is kept under behind the tile, parts (1, or the
+                  // tile's pages)
+  float4 ks;      // several pages: key scale of each 16 keys
+  float grow[4];  // and, where it has parts, what O is multiplied by before each
 };
 
 // Two CTAs have 113 KB each: with the converting warps' raw codes the ring of
@@ -66,9 +67,9 @@ template <bool Q8, int D>
 struct TilesLayout {
   static constexpr int KB = D / 64;
   static constexpr int RING = Q8 && D == 128 ? 3 : 4;
-  static constexpr int RAW = D == 128 ? 1 : 2;               // tiles of keys, and of values, whose codes are on their way
-  static constexpr int ROWS = KN / CVT_WARPS;                // of a tile, for each converting warp
-  static constexpr int RAW_BYTES = 2 * ROWS * D + 256;       // their codes (keys, values), then two scales a lane
+  static constexpr int RAW = D == 128 ? 1 : 2;               // a converting warp's tiles whose codes are on their way
+  static constexpr int ROWS = KN / (CVT_WARPS / 2);          // of a tile, for each of them
+  static constexpr int RAW_BYTES = ROWS * D + 256;           // their codes, then two scales a lane
   static constexpr int Q_BYTES = QM * D * 2;
   static constexpr int T_BYTES = KN * D * 2;
   static constexpr int OFF_RING = Q_BYTES;
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
       const int i = lane;
       const bool soft = i == B_QREADY || i == B_PFULL || i == B_PFULL + 1;
       const bool full = i >= B_RFULL && i < B_RFULL + MAX_RING;
-      mbar_init(bar(i), soft ? SOFT_WARPS : full && Q8 ? CVT_WARPS : 1);
+      mbar_init(bar(i), soft ? SOFT_WARPS : full && Q8 ? CVT_WARPS / 2 : 1);
     }
     static_assert(N_BARS <= 32, "a lane each");
     fence_barrier_init();
@@ -259,7 +260,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
         }
         const uint64_t dv = smem_desc_sw128_mn(ring_addr(n), KN * 128, 1024);
         const uint32_t pa = tmem + 64u * (uint32_t)buf;
-        const int parts = Q8 ? info(t)->parts : 1;
+        const int parts = Q8 ? (int)info(t)->head.w : 1;
         const int part_shift = parts == 1 ? 2 : parts == 2 ? 1 : 0;  // of 16-key steps
         for (int j = 0; j < parts && ok; ++j) {
           ok = wwait(B_PFULL + buf, (pf >> buf) & 1u);
@@ -350,10 +351,11 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
       const int buf = t & 1, k0 = (t0 + t) * KN;
       if (!(ok = wwait(B_SFULL + buf, (uint32_t)(t >> 1) & 1u))) break;
       tc_fence_after();
-      TileInfo ti{};
+      float4 ti = make_float4(1.f, 1.f, 0.f, 1.f), ks4 = ti;
       if constexpr (Q8) {
         if (!(ok = wwait(B_INFO + t % RING, (uint32_t)(t / RING) & 1u))) break;
-        ti = *info(t);
+        ti = info(t)->head;
+        if (np > 1) ks4 = info(t)->ks;
       }
       float x[KN];
       {
@@ -370,10 +372,10 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
       float c = rs;
       if constexpr (Q8) {
         if (np == 1) {
-          c = fmaxf(c * ti.ks[0], kTiny);
+          c = fmaxf(c * fabsf(ti.x), kTiny);
         } else {
 #pragma unroll
-          for (int j = 0; j < KN; ++j) x[j] *= ti.ks[j >> 4];
+          for (int j = 0; j < KN; ++j) x[j] *= fabsf(j < 16 ? ks4.x : j < 32 ? ks4.y : j < 48 ? ks4.z : ks4.w);
         }
       }
       if (k0 + KN > vmin) {
@@ -382,11 +384,16 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
           if (k0 + j >= vis) x[j] = -INFINITY;
       }
       if constexpr (Q8) {
-        if (fminf(fminf(ti.ks[0], ti.ks[1]), fminf(ti.ks[2], ti.ks[3])) < 0.f) {  // pages that are none are not seen
+        // pages that are none are not seen
+        if (np == 1) {
+          if (ti.x < 0.f) {
+#pragma unroll
+            for (int j = 0; j < KN; ++j) x[j] = -INFINITY;
+          }
+        } else if (fminf(fminf(ks4.x, ks4.y), fminf(ks4.z, ks4.w)) < 0.f) {
 #pragma unroll
           for (int j = 0; j < KN; ++j)
-            if (ti.ks[j >> 4] < 0.f) x[j] = -INFINITY;
-          c = rs;
+            if ((j < 16 ? ks4.x : j < 32 ? ks4.y : j < 48 ? ks4.z : ks4.w) < 0.f) x[j] = -INFINITY;
         }
       }
       // (three-way maxima; a NaN is passed over here and makes its weight one)
@@ -420,10 +427,10 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
       lsum += total.x + total.y;
       tmem_st32(trow + 64u * buf, pk);
       // ---- O: the row's maximum moved, or the reference of the values did
-      const int parts = Q8 ? ti.parts : 1;
+      const int parts = Q8 ? (int)ti.w : 1;
 #pragma unroll 1
       for (int j = 0; j < parts && ok; ++j) {
-        const float f = (j == 0 ? alpha : 1.f) * (Q8 ? ti.grow[j] : 1.f);
+        const float f = j == 0 ? alpha * ti.y : info(t)->grow[j];
         const bool scale = pv_buf >= 0 && __any_sync(0xffffffffu, f != 1.f);
         // (a part that is not the tile's first also waits because its arrival
         // below must not count for the part before)
@@ -437,7 +444,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
         pv_par = (pvw >> buf) & 1u;
         pvw ^= 1u << buf;
       }
-      if constexpr (Q8) ref = ti.ref;
+      if constexpr (Q8) ref = ti.z;
     }
     if (ok) ok = o_settled();
     // ---- O / l, through this warp's rows of the Q tile (every product that
@@ -509,68 +516,155 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
     }
   } else {
     // ------------------------------------------------------------ 8-bit converters
-    // Each of the warps takes its share of a tile's 64 rows, and all keep the
-    // same account of pages and scales (lane j < np: the tile's page j).
+    // Two warps turn the keys, 32 of a tile's 64 rows each, two the values,
+    // which also keep the account of the pages' scales.
     if constexpr (Q8) {
       const Kv8& cc = a.cache;
-      const int w = warp - 1 - SOFT_WARPS;
+      const int w = warp - LOAD_WARP;
+      const bool values = w >= CVT_WARPS / 2;
       constexpr int ROWS = L::ROWS, LR = D / 16, RI = 32 / LR, IT = ROWS / RI;  // lanes a row, rows an iteration, iterations
       constexpr int RAW = L::RAW;
-      const int r_in = lane / LR, ch = lane % LR;
-      const int shift = __ffs(page) - 1;  // of a page in tokens
+      const int ch = lane % LR;
+      const int row_first = ROWS * (w % (CVT_WARPS / 2)) + lane / LR;  // this lane's rows of a tile: it, + RI, ...
+      const int shift = __ffs(page) - 1;                               // of a page in tokens
       // a lane's own codes and scales, copied RAW tiles ahead of their use
       uint8_t* raw = sm + L::OFF_RAW + w * RAW * L::RAW_BYTES + lane * 16;
-      uint8_t* raw_sc = sm + L::OFF_RAW + w * RAW * L::RAW_BYTES + 2 * ROWS * D + lane * 8;
-      const int row_first = ROWS * w + r_in;  // this lane's rows of a tile: it, + RI, ...
-      auto page_id = [&](int t) -> int {      // lane j: the tile's page j
-        const int key = (t0 + t) * KN + (lane << shift);
-        return lane < np && t < nT && key < vmax ? cc.table[(long long)b * cc.table_ld + (key >> shift)] : -1;
+      uint8_t* raw_sc = sm + L::OFF_RAW + w * RAW * L::RAW_BYTES + ROWS * D + lane * 8;
+      // (a tile in one page: every lane knows that page; else lane j the tile's page j)
+      const bool one = np == 1;
+      const int my_page = one ? 0 : lane << shift, n_pages = cc.n_pages;
+      const int* table = cc.table + (long long)b * cc.table_ld;
+      auto page_id = [&](int t) -> int {
+        const int key = (t0 + t) * KN + my_page;
+        return (one || lane < np) && t < nT && key < vmax ? table[key >> shift] : -1;
       };
-      // ask for a tile's codes, keys (x = 0) or values
-      auto ask = [&](int x, int t, int ids) {
-        if (t < 0 || t >= nT) return;
-        const uint8_t* pool = x ? cc.v : cc.k;
-        const uint32_t dst = smem_u32(raw) + (t % RAW) * L::RAW_BYTES + x * ROWS * D;
-        const int key0 = (t0 + t) * KN;
-        const int id0 = __shfl_sync(0xffffffffu, ids, 0);
-        if (np == 1 && key0 + KN <= vmax && id0 >= 0 && id0 < cc.n_pages) {  // a whole tile of one page
-          const uint8_t* src =
-              pool + ((((long long)id0 * cc.n_kv_heads + h) << shift) + (key0 & (page - 1)) + row_first) * D + ch * 16;
+      auto is_page = [&](int id) { return (unsigned)id < (unsigned)n_pages; };
+      // this lane's first codes of page 0 of this head; bytes from page to page
+      const long long page_bytes = ((long long)cc.n_kv_heads << shift) * D;
+      const uint8_t* const base = (values ? cc.v : cc.k) + ((long long)h << shift) * D + ch * 16;
+      // ask for a tile's codes, and for the scales
+      auto ask = [&](int t, int ids) {
+        if (t < nT) {
+          uint8_t* sc = raw_sc + (t % RAW) * L::RAW_BYTES;
+          const uint32_t dst = smem_u32(raw) + (t % RAW) * L::RAW_BYTES;
+          const int key0 = (t0 + t) * KN;
+          const bool on = is_page(ids);
+          if (values) {
+            if (on) {
+              const long long ph = (long long)ids * cc.n_kv_heads + h;
+              cp_async4(smem_u32(sc), cc.k_scale + ph);
+              cp_async4(smem_u32(sc) + 4, cc.v_scale + ph);
+            } else {
+              *reinterpret_cast<float2*>(sc) = make_float2(-1.f, 1.f);
+            }
+          }
+          if (one && key0 + KN <= vmax && on) {  // a whole tile of one page
+            const uint8_t* src = base + (long long)ids * page_bytes + ((key0 & (page - 1)) + row_first) * D;
 #pragma unroll
-          for (int j = 0; j < IT; ++j) cp_async16(dst + j * 512, src + j * (RI * D), 16);
-        } else {
+            for (int j = 0; j < IT; ++j) cp_async16(dst + j * 512, src + j * (RI * D), 16);
+          } else {
 #pragma unroll
-          for (int j = 0; j < IT; ++j) {
-            const int r = row_first + j * RI, key = key0 + r;
-            const int id = __shfl_sync(0xffffffffu, ids, r >> shift);
-            const bool in = key < vmax && id >= 0 && id < cc.n_pages;
-            const uint8_t* src =
-                pool + ((((long long)(in ? id : 0) * cc.n_kv_heads + h) << shift) + (key & (page - 1))) * D + ch * 16;
-            cp_async16(dst + j * 512, src, in ? 16 : 0);
+            for (int j = 0; j < IT; ++j) {
+              const int r = row_first + j * RI, key = key0 + r;
+              const int id = __shfl_sync(0xffffffffu, ids, r >> shift);
+              const bool in = key < vmax && is_page(id);
+              cp_async16(dst + j * 512, base + (in ? id * page_bytes + (key & (page - 1)) * D : 0), in ? 16 : 0);
+            }
           }
         }
+        cp_commit();
       };
-      auto ask_scales = [&](int t, int ids) {
-        if (t >= nT) return;
-        uint8_t* sc = raw_sc + (t % RAW) * L::RAW_BYTES;
-        if (ids >= 0 && ids < cc.n_pages) {
-          const long long ph = (long long)ids * cc.n_kv_heads + h;
-          cp_async4(smem_u32(sc), cc.k_scale + ph);
-          cp_async4(smem_u32(sc) + 4, cc.v_scale + ph);
-        } else {
-          *reinterpret_cast<float2*>(sc) = make_float2(-1.f, 1.f);
-        }
-      };
-      // codes to f16 into the ring's next place: 16-byte chunks 2 ch and
-      // 2 ch + 1 of the row (the other one first in the second half of the
-      // row: fewer bank conflicts), times 2^dv of the row's page
-      int place = 0;
-      uint32_t lap = 1;  // parity of the place's last release
       const int c0 = (2 * ch) & 7, flip = (ch >> 2) & 1;
-      auto put = [&](const uint4 (&codes)[IT], int dv) -> bool {
-        if (!wwait(B_REMPTY + place, lap)) return false;
+      int ref = 0;
+      bool ok = true;
+      int id_next = page_id(0);
+#pragma unroll
+      for (int t = 0; t < RAW; ++t) {
+        const int id = id_next;
+        id_next = page_id(t + 1);
+        ask(t, id);
+      }
+#pragma unroll 1
+      for (int t = 0; t < nT && ok; ++t) {
+        cp_wait<RAW - 1>();
+        uint4 codes[IT];
+        const uint8_t* from = raw + (t % RAW) * L::RAW_BYTES;
+#pragma unroll
+        for (int j = 0; j < IT; ++j) codes[j] = *reinterpret_cast<const uint4*>(from + j * 512);
+        const float2 sc = *reinterpret_cast<const float2*>(raw_sc + (t % RAW) * L::RAW_BYTES);
+        {
+          const int id = id_next;
+          id_next = page_id(t + RAW + 1);
+          ask(t + RAW, id);
+        }
+        int dv = 0;  // exponent of the values' factor, lane j: of the tile's page j
+        if (values) {
+          // ---- the tile's scales
+          const float ks = sc.x;
+          const int ev = ((__float_as_int(sc.y) >> 23) & 255) - 127;
+          const bool in = one || (lane < np && (t0 + t) * KN + my_page < vmax);
+          const bool none = in && ks < 0.f;
+          if (none) report_error(a.err, DEV_ERR_BAD_SHAPE);
+          float grow = 1.f;  // of part j in lane j
+          int parts = 1;
+          if (one) {
+            if (none) {  // no values
+            } else if (t > 0 && ev - ref <= 7 && ev - ref >= -15) {
+              dv = ev - ref;
+            } else {
+              grow = t > 0 ? pow2i(ref - ev) : 1.f;
+              ref = ev;
+            }
+          } else {
+            const bool counts = in && !none;
+            const int mx = __reduce_max_sync(0xffffffffu, counts ? ev : -1000);
+            const int mn = __reduce_min_sync(0xffffffffu, counts ? ev : 1000);
+            if (mx == -1000) {  // no values
+            } else if (t > 0 && mx - ref <= 7 && mn - ref >= -15) {
+              dv = counts ? ev - ref : 0;  // (0: no values there)
+            } else if (mx - mn <= 15) {
+              grow = t > 0 ? pow2i(ref - mx) : 1.f;
+              ref = mx;
+              dv = counts ? ev - ref : 0;
+            } else {
+              // each counting page under its own reference; from which one O
+              // comes to it: the last counting page before, or the tile before
+              parts = np;
+              const uint32_t have = __ballot_sync(0xffffffffu, counts);
+              const uint32_t before = have & ((1u << lane) - 1u);
+              const int last = 31 - __clz(have);
+              const int prev = __shfl_sync(0xffffffffu, ev, before ? 31 - __clz(before) : 0);
+              grow = !counts ? 1.f : before ? pow2i(prev - ev) : t > 0 ? pow2i(ref - ev) : 1.f;
+              ref = __shfl_sync(0xffffffffu, ev, last);
+            }
+          }
+          if (w == CVT_WARPS / 2) {
+            // (info t - RING was read before P V of t - 3, which had to be done
+            // for the place of values t - 1, or of keys t - 1 before it)
+            TileInfo* ti = info(t);
+            if (!one) {
+              const int j = lane < 4 ? (lane * 16) >> shift : 0;
+              const float ks_j = __shfl_sync(0xffffffffu, ks, j);
+              const bool in_j = __shfl_sync(0xffffffffu, (int)in, j);
+              if (lane < 4) {
+                reinterpret_cast<float*>(&ti->ks)[lane] = in_j ? ks_j : 1.f;  // (keys behind the last are masked)
+                ti->grow[lane] = grow;
+              }
+              __syncwarp();
+            }
+            if (lane == 0) {
+              ti->head = make_float4(ks, grow, (float)ref, (float)parts);
+              mbar_arrive(bar(B_INFO + t % RING));
+            }
+          }
+        }
+        // ---- codes to f16 into the ring: 16-byte chunks 2 ch and 2 ch + 1 of
+        // the row (the other one first in the second half of the row: fewer
+        // bank conflicts), times 2^dv of the row's page
+        const int n = values ? at_v(t, nT) : at_k(t), place = n % RING;
+        if (!(ok = wwait(B_REMPTY + place, ((uint32_t)(n / RING) & 1u) ^ 1u))) break;
         uint8_t* tile = sm + L::OFF_RING + place * L::T_BYTES + (ch >> 2) * KN * 128 + row_first * 128;
-        const bool scaled = __any_sync(0xffffffffu, dv != 0);
+        const bool scaled = one ? dv != 0 : __any_sync(0xffffffffu, dv != 0);
 #pragma unroll
         for (int j = 0; j < IT; ++j) {
           const int r = row_first + j * RI;
@@ -583,7 +677,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
                 : "=r"(f[2 * e]), "=r"(f[2 * e + 1])
                 : "r"(cw[e]));
           if (scaled) {
-            const __half2 m = __float2half2_rn(pow2i(__shfl_sync(0xffffffffu, dv, r >> shift)));
+            const __half2 m = __float2half2_rn(pow2i(one ? dv : __shfl_sync(0xffffffffu, dv, r >> shift)));
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               __half2 y = __hmul2(*reinterpret_cast<__half2*>(&f[e]), m);
@@ -598,104 +692,6 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_RFULL + place));
-        if (++place == RING) place = 0, lap ^= 1u;
-        return true;
-      };
-      // step t turns keys t and values t - 1, and asks for keys t + RAW and
-      // values t + RAW - 1
-      int id_k = page_id(0), id_v = -1;  // pages of the tiles asked for next
-      int ref = 0, dv_cur = 0, dv_prev = 0;  // exponents of the values' factors, lane j: page j of tiles t, t - 1
-      bool ok = true;
-#pragma unroll 1
-      for (int t = -RAW; t <= nT && ok; ++t) {
-        uint4 kc[IT], vc[IT];
-        float ks = 1.f, vs = 1.f;
-        if (t >= 0) {
-          cp_wait<RAW - 1>();
-          const uint8_t* kr = raw + (t % RAW) * L::RAW_BYTES;
-          const uint8_t* vr = raw + ((t + RAW - 1) % RAW) * L::RAW_BYTES + ROWS * D;
-#pragma unroll
-          for (int j = 0; j < IT; ++j) {
-            kc[j] = *reinterpret_cast<const uint4*>(kr + j * 512);
-            vc[j] = *reinterpret_cast<const uint4*>(vr + j * 512);
-          }
-          const float2 sc = *reinterpret_cast<const float2*>(raw_sc + (t % RAW) * L::RAW_BYTES);
-          ks = sc.x;
-          vs = sc.y;
-        }
-        const int id_next = page_id(t + RAW + 1);
-        ask(0, t + RAW, id_k);
-        ask_scales(t + RAW, id_k);
-        ask(1, t + RAW - 1, id_v);
-        cp_commit();
-        id_v = id_k;
-        id_k = id_next;
-        if (t < 0) continue;
-        dv_prev = dv_cur;
-        if (t < nT) {
-          // ---- the tile's scales
-          const bool in = lane < np && (t0 + t) * KN + (lane << shift) < vmax;
-          const bool none = in && ks < 0.f;
-          if (none) report_error(a.err, DEV_ERR_BAD_SHAPE);
-          const int ev = ((__float_as_int(vs) >> 23) & 255) - 127;
-          float grow = 1.f;  // of part j in lane j
-          int parts = 1;
-          if (np == 1) {
-            const int e0 = __shfl_sync(0xffffffffu, none ? -1000 : ev, 0);
-            dv_cur = 0;
-            if (e0 == -1000) {  // no page: no values
-            } else if (t > 0 && e0 - ref <= 7 && e0 - ref >= -15) {
-              dv_cur = e0 - ref;
-            } else {
-              grow = t > 0 ? pow2i(ref - e0) : 1.f;
-              ref = e0;
-            }
-          } else {
-            const bool counts = in && !none;
-            const int mx = __reduce_max_sync(0xffffffffu, counts ? ev : -1000);
-            const int mn = __reduce_min_sync(0xffffffffu, counts ? ev : 1000);
-            if (mx == -1000) {
-              dv_cur = 0;
-            } else if (t > 0 && mx - ref <= 7 && mn - ref >= -15) {
-              dv_cur = counts ? ev - ref : 0;  // (0: no values there)
-            } else if (mx - mn <= 15) {
-              grow = t > 0 ? pow2i(ref - mx) : 1.f;
-              ref = mx;
-              dv_cur = counts ? ev - ref : 0;
-            } else {
-              // each counting page under its own reference; from which one O
-              // comes to it: the last counting page before, or the tile before
-              parts = np;
-              const uint32_t have = __ballot_sync(0xffffffffu, counts);
-              const uint32_t before = have & ((1u << lane) - 1u);
-              const int last = 31 - __clz(have);
-              const int from = __shfl_sync(0xffffffffu, ev, before ? 31 - __clz(before) : 0);
-              grow = !counts ? 1.f : before ? pow2i(from - ev) : t > 0 ? pow2i(ref - ev) : 1.f;
-              ref = __shfl_sync(0xffffffffu, ev, last);
-              dv_cur = 0;
-            }
-          }
-          if (w == 0) {
-            // (info t's place was read before values t - RING + 1 were released)
-            const int j = lane < 4 ? (lane * 16) >> shift : 0;
-            const float ks_j = __shfl_sync(0xffffffffu, ks, j);
-            const bool in_j = __shfl_sync(0xffffffffu, (int)in, j);
-            if (!(ok = wwait(B_REMPTY + place, lap))) break;
-            TileInfo* ti = info(t);
-            if (lane < 4) {
-              ti->ks[lane] = in_j ? ks_j : 1.f;  // (keys behind the last are masked)
-              ti->grow[lane] = grow;
-            }
-            if (lane == 0) {
-              ti->ref = (float)ref;
-              ti->parts = parts;
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(B_INFO + t % RING));
-          }
-          if (!(ok = put(kc, 0))) break;
-        }
-        if (t > 0) ok = put(vc, dv_prev);
       }
       cp_wait<0>();
     }
