@@ -11,25 +11,28 @@
 // Within a row the order is that of the logits, so each CTA reads its row (or
 // its part of one) once from memory and keeps the K largest as keys (ordered
 // value bits over the inverted index); only between rows do the sums matter.
-// Those are kept in f64, and the scores are compared in f64: two hypotheses a few f32 steps apart come out in the order
-// of their exact scores. A cluster holds one item: its CTAs put their lists
-// into the first one's shared memory, which joins them, so there is one launch
-// and no workspace.
+// Those are kept in f64, and the scores are compared in f64: two hypotheses a
+// few f32 steps apart come out in the order of their exact scores. A cluster
+// holds one item: its CTAs put their lists into the first one's shared memory,
+// which joins them, so there is one launch and no workspace.
 //
 // The K largest: the first pass leaves each thread's largest value; each warp
-// sorts its lanes' and takes the K-th, a value that K elements reach; the
-// largest of these bounds leaves a few dozen candidates, which the second pass
-// (out of the L1 cache) gathers and which are put in order by counting. Where
-// ties leave too many of them, the keys are taken one after another.
+// sorts its lanes'. K elements reach a warp's K-th, and the least of four warps'
+// (K / 4)-th: the largest of these bounds leaves about 2 K candidates, which the
+// second pass (out of the L1 cache) gathers and which are put in order by
+// counting. (With the first bound alone they were 120 for K = 16 and 700 for
+// K = 32.) Where ties leave too many, those above the bound and the first of the
+// equal ones are taken.
 //
-// Measured: 64 items of 8 rows of 8193 f32 logits 14 us (17 MB, 19% of the copy
-// rate), one item of 4 rows of 1025 5.6 us. Bound by the chain load -> sum ->
-// bound -> gather -> order -> cluster barrier -> K choices, 9 us for one item of
-// 8 rows, of which all CTAs run at once. Blocks of 8192 elements in registers
-// with all threads' maxima counted against each other took 120 us; the choice
-// by counting all K * K candidates 3 us more.
+// Measured: 64 items of 8 rows of 8193 f32 logits 12.2 us (17 MB, 21% of the copy
+// rate), one item of 4 rows of 1025 5.1 us. Bound by the chain load -> sum ->
+// bound -> gather -> order -> cluster barrier -> K choices, 5.5 us for one item of
+// 8 rows of 1025, and the start of 512 CTAs in clusters, 8.6 us for 64 such items.
+// Blocks of 8192 elements in registers with all threads' maxima counted against
+// each other took 120 us; the choice by counting all K * K candidates 3 us more.
 #include "common.cuh"
 #include "decode.h"
+#include "per_device.h"
 
 namespace pkc {
 
@@ -37,12 +40,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kCap = 512;  // candidates at most
-constexpr int kMaxCluster = 8;
+constexpr int kCap = 1024;  // candidates at most
 
-// Larger keys for larger values, and for the lower index among equal values.
+// Larger keys for larger values, and for the lower index among equal values
+// (-0 + 0 is +0: the zeros are equal).
 __device__ __forceinline__ unsigned long long make_key(float x, unsigned int idx) {
-  unsigned int u = __float_as_uint(x);
+  unsigned int u = __float_as_uint(x + 0.f);
   u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
   return ((unsigned long long)u << 32) | (0xffffffffu - idx);
 }
@@ -52,51 +55,38 @@ __device__ __forceinline__ float key_value(unsigned long long k) {
 }
 __device__ __forceinline__ int key_index(unsigned long long k) { return (int)(0xffffffffu - (unsigned int)k); }
 
-// A thread's share of row[v0 .. v1): f(values, first index, how many, index
-// step) for VE elements at a time, missing ones -inf. Which thread takes which
-// element, and so the order of the sums, goes by the index alone and is the
-// same for every row of a call: equal rows have equal sums, to the bit, and tie.
-// Aligned: every row of the call starts on 16 bytes (v0 a multiple of VE).
-template <typename T, bool ALIGNED, typename F>
+template <typename T>
+__device__ __forceinline__ float to_float(T x) {
+  if constexpr (sizeof(T) == 4)
+    return x;
+  else
+    return from_h(x);
+}
+
+// A thread's share of row[v0 .. v1), every kThreads-th element: f(values, first
+// index, how many) for VE of them at a time, missing ones -inf. Which thread
+// takes which element, and so the order of the sums, goes by the index alone:
+// equal rows have equal sums, to the bit, and tie, however they are aligned.
+// Reads of single elements, 16 on their way at a time: 3 of 16 rows of 50736 f32
+// logits 22 us; reads of 16 bytes, of which the registers hold fewer ahead, 33 us.
+template <typename T, typename F>
 __device__ __forceinline__ void each_group(const T* row, int v0, int v1, F&& f) {
   constexpr int VE = 16 / sizeof(T);
-  auto value = [](T x) -> float {
-    if constexpr (sizeof(T) == 4)
-      return x;
-    else
-      return from_h(x);
-  };
-  if constexpr (ALIGNED) {
-#pragma unroll 4
-    for (int v = v0 + threadIdx.x * VE; v < v1; v += kThreads * VE) {
-      float x[VE];
-      const int n = min(VE, v1 - v);
-      if (n == VE) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(row + v);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  constexpr int U = 16 / VE, STEP = kThreads * VE;  // 16 reads on their way
+  for (int v4 = v0 + threadIdx.x; v4 < v1; v4 += U * STEP) {
+    float x[U][VE];
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          if constexpr (sizeof(T) == 4) {
-            x[e] = __uint_as_float(w[e]);
-          } else {
-            const uint32_t u = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
-            x[e] = is_bf16<T>::value ? __uint_as_float(u << 16) : __half2float(__ushort_as_half((unsigned short)u));
-          }
-        }
-      } else {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < VE; ++e) x[e] = e < n ? value(row[v + e]) : -INFINITY;
+      for (int e = 0; e < VE; ++e) {
+        const int v = v4 + u * STEP + e * kThreads;
+        x[u][e] = v < v1 ? to_float(row[v]) : -INFINITY;
       }
-      f(x, v, n, 1);
-    }
-  } else {
-#pragma unroll 2
-    for (int v = v0 + threadIdx.x; v < v1; v += kThreads * VE) {
-      float x[VE];
-      const int n = min(VE, (v1 - v + kThreads - 1) / kThreads);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) x[e] = e < n ? value(row[v + e * kThreads]) : -INFINITY;
-      f(x, v, n, kThreads);
+    for (int u = 0; u < U; ++u) {
+      const int v = v4 + u * STEP;
+      if (v >= v1) break;
+      f(x[u], v, min(VE, (v1 - v + kThreads - 1) / kThreads));
     }
   }
 }
@@ -116,7 +106,7 @@ struct SelectShared {
   unsigned long long list[kCap];
   unsigned long long best[kMaxBeams];
   double sum[kWarps];
-  float max[kWarps], bound[kWarps];
+  float max[kWarps], bound[kWarps], fourth[kWarps];
   int count;
 };
 
@@ -151,8 +141,8 @@ __device__ void order_list(const unsigned long long* list, int n, int K, unsigne
   }
 }
 
-// K-th largest of the warp's 32 values (bitonic sort, descending)
-__device__ __forceinline__ float warp_kth(float v, int K) {
+// The warp's 32 values in order (bitonic sort, descending)
+__device__ __forceinline__ float warp_sort(float v) {
   unsigned int x = ordered(v);
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -163,14 +153,14 @@ __device__ __forceinline__ float warp_kth(float v, int K) {
       const bool up = ((lane & k) == 0) == ((lane & j) == 0);  // this lane keeps the larger
       x = up ? max(x, y) : min(x, y);
     }
-  return unordered(__shfl_sync(0xffffffffu, x, K - 1));
+  return unordered(x);
 }
 
 // exp(x - base) for base >= x: the special-function unit's error, 2^-22, and
 // 2^-24 of the exponent
 __device__ __forceinline__ float exp_below(float x, float base) { return ex2_approx((x - base) * 1.44269504f); }
 
-template <typename T, bool ALIGNED>
+template <typename T>
 __device__ void scan_part(SelectShared& sh, const T* row, int v0, int v1, int K) {
   constexpr int VE = 16 / sizeof(T);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -178,26 +168,25 @@ __device__ void scan_part(SelectShared& sh, const T* row, int v0, int v1, int K)
   // ---- pass 1: the largest value and the sum (a NaN or +inf makes it NaN)
   constexpr float kLowest = -3.402823466e38f;
   float tmax = kLowest;
-  double tsum = 0.0;
-  each_group<T, ALIGNED>(row, v0, v1, [&](const float (&x)[VE], int, int, int) {
+  double part[4] = {0.0, 0.0, 0.0, 0.0};  // (four sums: an addition in f64 takes long)
+  each_group<T>(row, v0, v1, [&](const float (&x)[VE], int, int) {
     float m = x[0];
 #pragma unroll
     for (int e = 1; e < VE; ++e) m = fmaxf(m, x[e]);
     if (m > tmax) {
-      tsum *= (double)exp_below(tmax, m);
+      const double f = (double)exp_below(tmax, m);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[e] *= f;
       tmax = m;
     }
     // each term into f64: next to the row's largest term a sum in f32 would
     // lose what tells two rows apart
-    double s0 = 0.0, s1 = 0.0;
 #pragma unroll
-    for (int e = 0; e < VE; e += 2) {
-      s0 += (double)exp_below(x[e], tmax);
-      s1 += (double)exp_below(x[e + 1], tmax);
-    }
-    tsum += s0 + s1;
+    for (int e = 0; e < VE; ++e) part[e & 3] += (double)exp_below(x[e], tmax);
   });
-  const float kth = warp_kth(tmax == kLowest ? -INFINITY : tmax, K);
+  const double tsum = (part[0] + part[1]) + (part[2] + part[3]);
+  const float sorted = warp_sort(tmax == kLowest ? -INFINITY : tmax);
+  const float kth = __shfl_sync(0xffffffffu, sorted, K - 1), fourth = __shfl_sync(0xffffffffu, sorted, (K + 3) / 4 - 1);
   float m = tmax;
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
@@ -206,42 +195,79 @@ __device__ void scan_part(SelectShared& sh, const T* row, int v0, int v1, int K)
   for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
   if (lane == 0) {
     sh.bound[warp] = kth;
+    sh.fourth[warp] = fourth;
     sh.max[warp] = m;
     sh.sum[warp] = s;
   }
   if (tid == 0) sh.count = 0;
   __syncthreads();
-  float bound = sh.bound[0];
+  // a value that K elements reach: K of one warp, or a quarter of K (rounded up)
+  // of each of four warps
+  float bound;
+  {
+    const float of_one = sh.bound[lane % kWarps], of_four = sh.fourth[lane % kWarps];
+    int above = 0;
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) bound = fmaxf(bound, sh.bound[w]);
-  // ---- pass 2: what reaches the bound (few threads hold any)
-  if (tmax >= bound || bound == -INFINITY) each_group<T, ALIGNED>(row, v0, v1, [&](const float (&x)[VE], int v, int n, int step) {
+    for (int w = 0; w < kWarps; ++w) above += sh.fourth[w] > of_four;
+    const unsigned int one = __reduce_max_sync(0xffffffffu, ordered(of_one));
+    const unsigned int four = __reduce_min_sync(0xffffffffu, above < 4 ? ordered(of_four) : 0xffffffffu);
+    bound = unordered(max(one, four));
+  }
+  // ---- pass 2: what reaches the bound (few threads hold any), no more than the
+  // list holds
+  if (tmax >= bound || bound == -INFINITY) each_group<T>(row, v0, v1, [&](const float (&x)[VE], int v, int n) {
     float m = x[0];
 #pragma unroll
     for (int e = 1; e < VE; ++e) m = fmaxf(m, x[e]);
-    if (m >= bound) {
+    if (m >= bound && *(volatile int*)&sh.count <= kCap) {
 #pragma unroll
       for (int e = 0; e < VE; ++e)
         if (e < n && x[e] >= bound) {
           const int at = atomicAdd(&sh.count, 1);
-          if (at < kCap) sh.list[at] = make_key(x[e], v + e * step);
+          if (at < kCap) sh.list[at] = make_key(x[e], v + e * kThreads);
         }
     }
   });
   __syncthreads();
-  const int n = sh.count;
+  int n = sh.count;
+  if (n > kCap) {
+    // many equal ones, as where a mask leaves few tokens: what is above the
+    // bound, then the first of those that equal it
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    each_group<T>(row, v0, v1, [&](const float (&x)[VE], int v, int cnt) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (e < cnt && x[e] > bound && *(volatile int*)&sh.count <= kCap) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kCap) sh.list[at] = make_key(x[e], v + e * kThreads);
+        }
+    });
+    __syncthreads();
+    n = sh.count;
+    for (int base = v0; n < K && base < v1; base += kThreads) {
+      __syncthreads();
+      if (base + tid < v1) {
+        const float x = to_float(row[base + tid]);
+        if (x == bound) sh.list[atomicAdd(&sh.count, 1)] = make_key(x, base + tid);
+      }
+      __syncthreads();
+      n = sh.count;
+    }
+  }
   if (n <= kCap) {
     order_list(sh.list, n, K, out.key);
   } else {
-    // too many equal values: the keys one after another, each the largest
-    // below the one before
+    // still too many: the keys one after another, each the largest below the
+    // one before
     unsigned long long before = ~0ull;
     for (int j = 0; j < K; ++j) {
       unsigned long long best = 0;
-      each_group<T, ALIGNED>(row, v0, v1, [&](const float (&x)[VE], int v, int cnt, int step) {
+      each_group<T>(row, v0, v1, [&](const float (&x)[VE], int v, int cnt) {
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-          const unsigned long long k = make_key(x[e], v + e * step);
+          const unsigned long long k = make_key(x[e], v + e * kThreads);
           if (e < cnt && x[e] == x[e] && k < before && k > best) best = k;
         }
       });
@@ -272,7 +298,7 @@ __device__ void scan_part(SelectShared& sh, const T* row, int v0, int v1, int K)
 }
 
 // chunks: parts of a row (CTA r takes part r % chunks of rows r / chunks, + C / chunks, ...)
-template <typename T, bool ALIGNED>
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) k_beam_select(const BeamSelectArgs a, int chunks) {
   __shared__ SelectShared sh;
   uint32_t C;
@@ -286,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_select(const BeamSelectArg
   const int chunk = rank % chunks, per = ((a.V + chunks - 1) / chunks + 7) / 8 * 8;
   for (int beam = rank / chunks; beam < K; beam += lanes) {
     const T* row = reinterpret_cast<const T*>(a.logits) + (long long)(b * (long long)K + beam) * a.ld;
-    scan_part<T, ALIGNED>(sh, row, min(a.V, chunk * per), min(a.V, (chunk + 1) * per), K);
+    scan_part<T>(sh, row, min(a.V, chunk * per), min(a.V, (chunk + 1) * per), K);
     // to the first CTA's part [beam][chunk], word by word
     if (!started) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all of them run
     started = true;
@@ -298,11 +324,11 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_select(const BeamSelectArg
   }
   if (!started) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   cluster_sync();  // every part has arrived
-  if (rank != 0 || tid >= 32) return;
-  // ---- the first warp takes the K best off the heads of the lists, a lane a
-  // list (K * chunks <= 32); the lowest lane among equal scores has the lowest
-  // beam and, of a row's parts, the lowest tokens
-  const int beam = tid / chunks;
+  if (rank != 0) return;
+  // ---- the scores of all K * chunks <= 32 lists, a lane a list, warps sharing
+  // the places: list[place][lane], ordered bits, 0 where the list has ended
+  static_assert(kCap >= 32 * kMaxBeams, "the scores lie where the candidates were");
+  const int lane = tid & 31, beam = lane / chunks;
   const bool on = beam < K;
   const Part* rows = &sh.part[on ? beam * chunks : 0];
   float m = -INFINITY;
@@ -315,51 +341,49 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_select(const BeamSelectArg
   // that offers nothing, its lowest tokens
   const int kind = cum != cum || cum == -INFINITY ? 2 : fin ? 1 : s > 0.0 && isfinite(s) && isfinite(m) ? 0 : 2;
   const double lse = (double)m + log(s);
-  const Part& mine = sh.part[on ? tid : 0];
-  const bool lists = on && (kind == 0 || tid % chunks == 0);
+  const Part& mine = sh.part[on ? lane : 0];
+  const bool lists = on && (kind == 0 || lane % chunks == 0);
   const int len = !lists ? 0 : kind == 0 ? mine.n : min(a.V, K);
-  int j = 0, tok = -1;
-  unsigned long long head = 0;  // ordered bits of the score; 0: the list is empty
-  auto next = [&]() {
-    head = 0;
-    if (j >= len) return;
+  for (int j = tid >> 5; j < K; j += kWarps) {
     double sc = -INFINITY;
-    if (kind == 0) {
-      const unsigned long long k = mine.key[j];
-      tok = key_index(k);
-      sc = (double)cum + ((double)key_value(k) - lse);
-    } else {
-      tok = kind == 2 ? j : j == 0 ? a.eos : j - 1 < a.eos ? j - 1 : j;
-      if (kind == 1 && j == 0) sc = (double)cum;
-    }
-    head = ordered(sc);
-    ++j;
-  };
-  next();
-  float score = 0.f;
-  int parent = 0, token = 0, done = 0;  // of place tid
+    if (kind == 0 && j < len) sc = (double)cum + ((double)key_value(mine.key[j]) - lse);
+    if (kind == 1 && j == 0) sc = (double)cum;
+    sh.list[j * 32 + lane] = j < len ? ordered(sc + 0.0) : 0;  // (+ 0: the zeros are equal)
+  }
+  __syncthreads();  // (cum and finished, which the outputs may be, have been read)
+  if (tid >= 32) return;
+  // ---- the first warp takes the K best off the lists' heads; the lowest lane
+  // among equal scores has the lowest beam and, of a row's parts, the lowest
+  // tokens. (Scores worked out as their lists' heads moved on: 1.2 us more for
+  // K = 8, 2.6 us for K = 16.)
+  unsigned long long head = sh.list[lane], best = 0;
+  int at = 0, list = 0, entry = 0;  // list, entry: of place lane
   for (int place = 0; place < K; ++place) {
     const unsigned int hi = (unsigned int)(head >> 32), top = __reduce_max_sync(0xffffffffu, hi);
     const unsigned int lo = hi == top ? (unsigned int)head : 0u, low = __reduce_max_sync(0xffffffffu, lo);
-    const int from = __ffs(__ballot_sync(0xffffffffu, hi == top && lo == low && head != 0)) - 1;
-    const unsigned long long best = ((unsigned long long)top << 32) | low;
-    const int t = __shfl_sync(0xffffffffu, tok, from), f = __shfl_sync(0xffffffffu, (int)fin, from);
-    if (tid == place) {
-      const double sc = __longlong_as_double((long long)((best >> 63) ? (best & ~(1ull << 63)) : ~best));
-      score = (float)sc;
-      parent = from / chunks;
-      token = t;
-      done = t == a.eos || f;
+    const int from = __ffs(__ballot_sync(0xffffffffu, hi == top && lo == low)) - 1;
+    const int e = __shfl_sync(0xffffffffu, at, from);
+    if (lane == place) {
+      best = ((unsigned long long)top << 32) | low;
+      list = from;
+      entry = e;
     }
-    if (tid == from) next();
+    if (lane == from) {
+      ++at;
+      head = at < K ? sh.list[at * 32 + lane] : 0;
+    }
   }
-  // (cum and finished, which these may be, have been read)
-  if (tid < K) {
-    const long long o = (long long)b * K + tid;
-    a.score[o] = score;
-    a.parent[o] = parent;
+  const int from_kind = __shfl_sync(0xffffffffu, kind, list), from_fin = __shfl_sync(0xffffffffu, (int)fin, list);
+  if (lane < K) {
+    const int token = from_kind == 0   ? key_index(sh.part[list].key[entry])
+                : from_kind == 2 ? entry
+                : entry == 0     ? a.eos
+                                 : (entry - 1 < a.eos ? entry - 1 : entry);
+    const long long o = (long long)b * K + lane;
+    a.score[o] = (float)__longlong_as_double((long long)((best >> 63) ? (best & ~(1ull << 63)) : ~best));
+    a.parent[o] = list / chunks;
     a.token[o] = token;
-    if (a.finished_out) a.finished_out[o] = (uint8_t)done;
+    if (a.finished_out) a.finished_out[o] = (uint8_t)(token == a.eos || from_fin);
   }
 }
 
@@ -423,13 +447,25 @@ cudaError_t reorder_v(const BeamReorderArgs& a, cudaStream_t st) {
   return launch_pdl(k_beam_reorder<V, 32>, grid, block, 0, st, a);
 }
 
-template <typename T, bool ALIGNED>
+template <typename T>
 cudaError_t select_t(const BeamSelectArgs& a, cudaStream_t st) {
-  // CTAs of an item: a row each, or parts of a row where there are few rows
-  // and the parts are not short
-  int chunks = 1;
-  while (a.K * chunks * 2 <= kMaxCluster && a.V >= chunks * 2 * 2048) chunks *= 2;
-  const int C = a.K * chunks < kMaxCluster ? a.K * chunks : kMaxCluster / chunks * chunks;
+  // CTAs of an item: a row each, or, where all rows together leave SMs without
+  // work, parts of at least 2048 elements of each. More than eight CTAs (which
+  // only some devices' clusters allow) where there are few items: 3 of 16 rows
+  // of 50736 logits 20 us, 34 with eight.
+  const long long rows = (long long)a.B * a.K;
+  const int most = rows < 2 * 148 ? 16 : 8;
+  int chunks = most / a.K;
+  if (chunks > a.V / 2048) chunks = a.V / 2048;
+  if (chunks > 2 * 148 / rows) chunks = (int)(2 * 148 / rows);
+  if (chunks < 1) chunks = 1;
+  const int C = a.K * chunks < most ? a.K * chunks : most / chunks * chunks;
+  static PerDevice once;
+  int unused = 0;
+  const cudaError_t ae = per_device(once, &unused, [&](int, int&) {
+    return cudaFuncSetAttribute(k_beam_select<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  });
+  if (ae != cudaSuccess) return ae;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.B * C));
   cfg.blockDim = dim3(kThreads);
@@ -442,17 +478,16 @@ cudaError_t select_t(const BeamSelectArgs& a, cudaStream_t st) {
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, k_beam_select<T, ALIGNED>, a, chunks);
+  return cudaLaunchKernelEx(&cfg, k_beam_select<T>, a, chunks);
 }
 
 }  // namespace
 
 cudaError_t beam_select_launch(const BeamSelectArgs& a, int dtype, cudaStream_t st) {
   if (a.B <= 0) return cudaSuccess;
-  const bool al = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.ld % (dtype == 2 ? 4 : 8) == 0;
-  if (dtype == 0) return al ? select_t<__half, true>(a, st) : select_t<__half, false>(a, st);
-  if (dtype == 1) return al ? select_t<__nv_bfloat16, true>(a, st) : select_t<__nv_bfloat16, false>(a, st);
-  return al ? select_t<float, true>(a, st) : select_t<float, false>(a, st);
+  if (dtype == 0) return select_t<__half>(a, st);
+  if (dtype == 1) return select_t<__nv_bfloat16>(a, st);
+  return select_t<float>(a, st);
 }
 
 cudaError_t beam_reorder_launch(const BeamReorderArgs& a, cudaStream_t st) {

@@ -632,6 +632,44 @@ def test_beam_select_ties(cuda, B, K, V):
     assert torch.equal(parent.long(), want // V) and torch.equal(token.long(), want % V)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("B,K,V,live", [(2, 5, 50736, 3), (1, 32, 9001, 20), (3, 8, 8193, 8), (2, 16, 700, 1),
+                                        (1, 4, 4096, 0)])
+@pytest.mark.parametrize("mask", ["lowest", "-inf", "-1e4"])
+def test_beam_select_masked_vocabulary(cuda, dtype, B, K, V, live, mask):
+    """A mask that leaves a row few tokens, fewer than K among them: the others
+    are all alike, and the lowest of them fill the places."""
+    import torch
+    g = torch.Generator().manual_seed(V + live)
+    dt = getattr(torch, dtype)
+    value = {"lowest": torch.finfo(dt).min, "-inf": float("-inf"), "-1e4": -1e4}[mask]
+    logits = torch.full((B, K, V), value, dtype=dt)
+    for b in range(B):
+        for k in range(K):
+            at = torch.randperm(V, generator=g)[:live]
+            logits[b, k, at] = torch.randn(live, generator=g).to(dt)
+    cum = torch.randn(B, K, generator=g) - 10
+    check_select(logits.to(cuda), cum.to(cuda), torch.zeros(B, K, dtype=torch.uint8, device=cuda), V - 1)
+
+
+def test_beam_select_zeros_of_either_sign(cuda):
+    """-0 and +0 are the same logit and the same score: the lowest index wins."""
+    import torch
+    B, K, V = 1, 4, 300
+    for dt in (torch.float32, torch.float16, torch.bfloat16):
+        logits = torch.zeros(B, K, V, dtype=dt, device=cuda)
+        logits[..., ::2] = -0.0
+        cum = torch.zeros(B, K, device=cuda)
+        cum[:, 0] = -0.0
+        no = torch.zeros(B, K, dtype=torch.uint8, device=cuda)
+        _, parent, token, _ = run_select(logits, cum, no, V - 1)
+        assert (parent == 0).all() and torch.equal(token.long(), torch.arange(K, device=cuda).expand(B, K))
+        # finished hypotheses with scores of either sign: the lower beam first
+        score, parent, token, _ = run_select(logits, cum, torch.ones_like(no), 7)
+        assert torch.equal(parent.long(), torch.arange(K, device=cuda).expand(B, K)) and (token == 7).all()
+        assert (score == 0).all()
+
+
 def test_beam_select_sorted_rows(cuda):
     """Ascending and descending rows, and the largest values all in one
     thread's share."""
