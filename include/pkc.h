@@ -429,10 +429,10 @@ pkc_status pkc_relpos_attention_noalloc(const void* qkv, const void* ptab, int c
    gives zeros. q, out [q_rows][n_heads][head_dim]; k, v
    [kv_rows][n_kv_heads][head_dim] (with row strides, so the k | v rows of one
    projection need no copy); q_off [B + 1], kv_off, kv_len [B] int32 on the
-   device. max_q and max_kv bound the items' rows and keys. All of an item's
-   hypotheses are its query rows: they share one read of its keys. workspace:
-   pkc_cross_attention_workspace bytes, 16-byte aligned (NULL if 0). out may
-   not overlap the inputs. */
+   device. max_q and max_kv (up to 2^30) bound the items' rows and keys. All of
+   an item's hypotheses are its query rows: they share one read of its keys.
+   workspace: pkc_cross_attention_workspace bytes, 16-byte aligned (NULL if 0).
+   out may not overlap the inputs. */
 pkc_status pkc_cross_attention(const void* q, long long ldq, const int* q_off, int max_q, int q_rows, const void* k,
                                long long ldk, const void* v, long long ldv, const int* kv_off, const int* kv_len,
                                int max_kv, int kv_rows, int B, int n_heads, int n_kv_heads, int head_dim, float scale,
@@ -471,7 +471,9 @@ pkc_status pkc_kv8_append(const pkc_kv8_cache* cache, const void* k, long long l
 /* Causal self attention over the cache: the query rows [q_off[s], q_off[s+1])
    are sequence s's last n tokens (appended before), so row i of n sees its
    first lens[s] - n + i + 1 tokens. Other arguments as
-   pkc_cross_attention; max_len bounds lens. */
+   pkc_cross_attention; max_len (up to 2^30) bounds lens. max_q also chooses
+   the kernel: sequences of many new tokens and of one are faster in a call
+   each. */
 pkc_status pkc_kv8_attention(const pkc_kv8_cache* cache, const void* q, long long ldq, const int* q_off, int max_q,
                              int q_rows, const int* lens, int max_len, int n_seqs, int n_heads, float scale, int dtype,
                              void* out, long long ldo, void* workspace, size_t workspace_bytes, int* err, void* stream);

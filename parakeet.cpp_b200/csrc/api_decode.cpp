@@ -27,6 +27,10 @@ pkc_status guarded(const char* what, F&& body) noexcept {
   }
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+// keys of one item: places of keys are ints, and rounded up to tiles
+constexpr int kMaxKeys = 1 << 30;
+
 pkc_status bad(const char* what, const char* why) {
   return pkc::set_thread_error(PKC_ERR_ARG, std::string(what) + ": " + why);
 }
@@ -121,11 +125,12 @@ extern "C" pkc_status pkc_cross_attention(const void* q, long long ldq, const in
   const char* what = "pkc_cross_attention";
   return guarded(what, [&]() -> pkc_status {
     if (B < 0 || q_rows < 0 || kv_rows < 0 || max_q < 0 || max_kv < 0) return bad(what, "a size is negative");
+    if (max_kv > kMaxKeys) return bad(what, "max_kv is more than 2^30");
     if (dtype != 0 && dtype != 1) return bad(what, "dtype must be 0 (f16) or 1 (bf16)");
     if (head_dim != 64 && head_dim != 128) return bad(what, "head_dim must be 64 or 128");
     if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads)
       return bad(what, "n_heads must be a positive multiple of n_kv_heads");
-    if (!std::isfinite(scale)) return bad(what, "scale must be finite");
+    if (!std::isfinite(scale * kLog2e)) return bad(what, "scale must be finite, and its product with log2(e)");
     if (B == 0 || max_q == 0 || q_rows == 0) return PKC_OK;
     if (!q || !q_off || !kv_off || !kv_len || !out || ((!k || !v) && kv_rows > 0)) return bad(what, "a pointer is NULL");
     const long long qr = (long long)n_heads * head_dim, kr = (long long)n_kv_heads * head_dim;
@@ -146,7 +151,7 @@ extern "C" pkc_status pkc_cross_attention(const void* q, long long ldq, const in
     a.k = k; a.v = v; a.ldk = ldk; a.ldv = ldv; a.kv_off = kv_off; a.kv_len = kv_len;
     a.max_kv = max_kv; a.kv_rows = kv_rows;
     a.n_items = B; a.n_heads = n_heads; a.n_kv_heads = n_kv_heads; a.head_dim = head_dim;
-    a.scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale * kLog2e;
     a.out = out; a.ldo = ldo; a.ws = static_cast<float*>(workspace); a.err = err;
     return launched(what, pkc::decode_attn_launch(a, dtype == 1, reinterpret_cast<cudaStream_t>(stream)));
   });
@@ -169,7 +174,8 @@ extern "C" pkc_status pkc_kv8_append(const pkc_kv8_cache* cache, const void* k, 
     const pkc_status ds = check_device(what, stream, {new_off, lens, cache->table, cache->k_scale, cache->v_scale, err},
                                        {k, v, cache->k, cache->v});
     if (ds != PKC_OK) return ds;
-    pkc::Kv8AppendArgs a{kv8_of(cache), k, v, ldk, ldv, new_off, lens, n_seqs, rows, max_new, err};
+    // (no sequence has more new tokens than there are)
+    pkc::Kv8AppendArgs a{kv8_of(cache), k, v, ldk, ldv, new_off, lens, n_seqs, rows, max_new < rows ? max_new : rows, err};
     return launched(what, pkc::kv8_append_launch(a, dtype == 1, reinterpret_cast<cudaStream_t>(stream)));
   });
 }
@@ -189,11 +195,12 @@ extern "C" pkc_status pkc_kv8_attention(const pkc_kv8_cache* cache, const void* 
   return guarded(what, [&]() -> pkc_status {
     if (const char* why = cache_fault(cache)) return bad(what, why);
     if (n_seqs < 0 || q_rows < 0 || max_q < 0 || max_len < 0) return bad(what, "a size is negative");
-    if (max_len > (long long)cache->table_ld * cache->page) return bad(what, "max_len is beyond the block table");
+    if (max_len > kMaxKeys || max_len > (long long)cache->table_ld * cache->page)
+      return bad(what, "max_len is more than 2^30 or beyond the block table");
     if (dtype != 0 && dtype != 1) return bad(what, "dtype must be 0 (f16) or 1 (bf16)");
     if (n_heads <= 0 || n_heads % cache->n_kv_heads)
       return bad(what, "n_heads must be a positive multiple of n_kv_heads");
-    if (!std::isfinite(scale)) return bad(what, "scale must be finite");
+    if (!std::isfinite(scale * kLog2e)) return bad(what, "scale must be finite, and its product with log2(e)");
     if (n_seqs == 0 || max_q == 0 || q_rows == 0) return PKC_OK;
     if (!q || !q_off || !lens || !out) return bad(what, "a pointer is NULL");
     const long long qr = (long long)n_heads * cache->head_dim;
@@ -211,7 +218,7 @@ extern "C" pkc_status pkc_kv8_attention(const pkc_kv8_cache* cache, const void* 
     a.q = q; a.ldq = ldq; a.q_off = q_off; a.max_q = max_q; a.q_rows = q_rows;
     a.kv_len = lens; a.max_kv = max_len; a.cache = kv8_of(cache);
     a.n_items = n_seqs; a.n_heads = n_heads; a.n_kv_heads = cache->n_kv_heads; a.head_dim = cache->head_dim;
-    a.scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale * kLog2e;
     a.out = out; a.ldo = ldo; a.ws = static_cast<float*>(workspace); a.err = err;
     return launched(what, pkc::decode_attn_launch(a, dtype == 1, reinterpret_cast<cudaStream_t>(stream)));
   });

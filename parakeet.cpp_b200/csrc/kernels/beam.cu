@@ -454,29 +454,38 @@ cudaError_t select_t(const BeamSelectArgs& a, cudaStream_t st) {
   // only some devices' clusters allow) where there are few items: 3 of 16 rows
   // of 50736 logits 20 us, 34 with eight.
   const long long rows = (long long)a.B * a.K;
-  const int most = rows < 2 * 148 ? 16 : 8;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  static PerDevice once;
+  int largest = 0;
+  const cudaError_t ae = per_device(once, &largest, [&](int, int& v) {
+    cudaError_t e = cudaFuncSetAttribute(k_beam_select<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    at[0].val.clusterDim.x = 16;
+    cfg.gridDim = dim3(16);
+    cfg.numAttrs = 1;
+    int n = 0;
+    e = cudaOccupancyMaxActiveClusters(&n, k_beam_select<T>, &cfg);
+    v = e == cudaSuccess && n > 0 ? 16 : 8;
+    if (e != cudaSuccess) cudaGetLastError();
+    return cudaSuccess;
+  });
+  if (ae != cudaSuccess) return ae;
+  const int most = rows < 2 * 148 ? largest : 8;
   int chunks = most / a.K;
   if (chunks > a.V / 2048) chunks = a.V / 2048;
   if (chunks > 2 * 148 / rows) chunks = (int)(2 * 148 / rows);
   if (chunks < 1) chunks = 1;
   const int C = a.K * chunks < most ? a.K * chunks : most / chunks * chunks;
-  static PerDevice once;
-  int unused = 0;
-  const cudaError_t ae = per_device(once, &unused, [&](int, int&) {
-    return cudaFuncSetAttribute(k_beam_select<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  });
-  if (ae != cudaSuccess) return ae;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.B * C));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = C;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
+  cfg.gridDim = dim3((unsigned)(a.B * C));
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, k_beam_select<T>, a, chunks);
 }

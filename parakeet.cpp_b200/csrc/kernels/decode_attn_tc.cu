@@ -76,7 +76,7 @@ struct TileInfo {
 // 128-column tiles has three places instead of four.
 template <bool Q8, int D>
 struct TilesLayout {
-  static constexpr int KB = D / 64;
+  [[maybe_unused]] static constexpr int KB = D / 64;
   static constexpr int RING = Q8 && D == 128 ? 3 : 4;
   static constexpr int RAW = D == 128 ? 1 : 2;               // a converting warp's tiles whose codes are on their way
   static constexpr int ROWS = KN / (CVT_WARPS / 2);          // of a tile, for each of them

@@ -95,6 +95,16 @@ def test_kv8_attention_refuses():
         refused(call, **kw)
 
 
+def test_attention_refuses_what_overflows():
+    import pkc
+    for scale in (3e38, -3e38):  # times log2(e): an infinity
+        assert "scale" in refused(cross, scale=scale)
+    assert "2^30" in refused(cross, max_kv=2 ** 30 + 1)
+    wide = cache(table_ld=2 ** 27)
+    assert "2^30" in refused(pkc.kv8_attention, wide, P, P, P, 1, 4, q_rows=1, max_q=1, max_len=2 ** 30 + 1, bf16=True, out=P)
+    assert "scale" in refused(pkc.kv8_attention, wide, P, P, P, 1, 4, q_rows=1, max_q=1, max_len=8, bf16=True, out=P, scale=3e38)
+
+
 def test_kv8_reorder_refuses():
     import pkc
     for args in ((0, P, 1, 2), (P, 0, 1, 2), (P, P, -1, 2), (P, P, 70000, 2), (P, P, 1, 0), (P, P, 1, 33), (P + 2, P, 1, 2), (P, P + 1, 1, 2)):

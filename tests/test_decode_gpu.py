@@ -326,6 +326,22 @@ def test_kv8_append_twice_is_once(cuda, n):
         assert torch.equal(c[x].view(torch.uint8), y.view(torch.uint8))
 
 
+@pytest.mark.parametrize("n", [1, 40])
+def test_kv8_append_loose_bound(cuda, n):
+    """max_new far above what comes writes the same bytes."""
+    import torch
+    g = torch.Generator().manual_seed(2)
+    new = torch.randn(2 * n, 2, 2, 64, generator=g).half().to(cuda)
+    got = []
+    for bound in (n, 2 ** 31 - 1):
+        c = make_cache(cuda, 2, [n, n], 2, 64, 16)
+        append(c, new, [n, n], [n, n], max_new=bound)
+        assert int(c["err"]) == 0
+        got.append([c[x].view(torch.uint8).clone() for x in ("k", "v", "k_scale", "v_scale")])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("n", [2, 20])
 def test_kv8_append_special_values(cuda, n):
     """Infinities take the largest code and set no scale, a NaN is stored as 0
