@@ -723,6 +723,37 @@ struct Plan {
   bool clustered;                       // the parts are joined in a cluster
   long long blocks;
 };
+// Parts of the keys for the tcgen05 kernel, of at least 256 keys; 2 * kSms CTAs
+// run at a time.
+//  - One item: the number that ends first, in tiles one after another, the start
+//    and the end of a part counted as six. 256 new tokens over 16384, 16 heads
+//    of 64 for 4: nine parts in one round 57 us, 19 in a little over two 74 us.
+//  - Several, whose lengths may differ: one round of CTAs, or two of parts of at
+//    least 512 keys over the 8-bit cache, whose tiles cost more (the 8-bit chunk
+//    180 us with one, 174 with two); one where that leaves the second mostly
+//    empty (three items of 8192, 8 heads for one: 48 instead of 62 us).
+int tile_parts(int n_items, long long blocks, int max_kv, bool q8) {
+  constexpr long long slots = 2LL * kSms;
+  const int tiles = max_kv / 64 + 1, most = max_kv / 256 < 1 ? 1 : max_kv / 256 > 64 ? 64 : max_kv / 256;
+  if (n_items == 1) {
+    int best = 1;
+    long long least = 0;
+    for (int n = 1; n <= most; ++n) {
+      const long long cost = (blocks * n + slots - 1) / slots * ((tiles + n - 1) / n + 6);
+      if (n == 1 || cost < least) best = n, least = cost;
+    }
+    return best;
+  }
+  if (blocks <= 0) return 1;
+  const long long fill = q8 ? 2 * slots : slots;
+  long long n = fill / blocks;
+  if (n < 4) n = (fill + blocks - 1) / blocks;
+  if (n > most) n = most;
+  if (blocks * n > slots && n > max_kv / 512) n = max_kv / 512;
+  if (4 * blocks <= slots && blocks * n > slots && 4 * blocks * n < 7 * slots) n = slots / blocks;
+  return n < 1 ? 1 : (int)n;
+}
+
 Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, bool q8, bool tiles = true) {
   Plan p;
   const long long rows = (long long)max_q * (n_heads / n_kv_heads);
@@ -732,13 +763,7 @@ Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, 
     p.blocks = (long long)n_items * n_kv_heads * p.row_tiles;
     p.warps = 0;
     p.clustered = false;
-    // parts of at least 512 keys (a part costs as much as six more tiles),
-    // until two CTAs run on every SM; twice as many over the 8-bit cache, whose
-    // tiles cost more, so that uneven lengths count more
-    const long long fill = (q8 ? 4LL : 2LL) * kSms;
-    const long long want = (fill + p.blocks - 1) / (p.blocks > 0 ? p.blocks : 1), most = max_kv / 512;
-    const long long n = want < most ? want : most;
-    p.n_split = n < 1 ? 1 : n > 64 ? 64 : (int)n;
+    p.n_split = tile_parts(n_items, p.blocks, max_kv, q8);
     return p;
   }
   p.rows = rows <= 8 ? 8 : 16;
@@ -749,7 +774,7 @@ Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, 
   p.n_split = 1;
   p.clustered = false;
   if (p.warps == 4 && tiles && p.blocks > 0) {
-    const long long most = (max_kv + 127) / 128, want = 2 * slots / (4 * p.blocks);  // two rounds of CTAs
+    const long long most = ((long long)max_kv + 127) / 128, want = 2 * slots / (4 * p.blocks);  // two rounds of CTAs
     const long long n0 = want < most ? want : most;
     p.clustered = n0 <= 8 || max_kv <= 8 * 1024;
     const long long n = p.clustered && n0 > 8 ? 8 : n0 > 64 ? 64 : n0;

@@ -76,13 +76,13 @@ struct TileInfo {
 // 128-column tiles has three places instead of four.
 template <bool Q8, int D>
 struct TilesLayout {
-  [[maybe_unused]] static constexpr int KB = D / 64;
+  static constexpr int KB = D / 64;
   static constexpr int RING = Q8 && D == 128 ? 3 : 4;
   static constexpr int RAW = D == 128 ? 1 : 2;               // a converting warp's tiles whose codes are on their way
   static constexpr int ROWS = KN / (CVT_WARPS / 2);          // of a tile, for each of them
   static constexpr int RAW_BYTES = ROWS * D + 256;           // their codes, then two scales a lane
   static constexpr int Q_BYTES = QM * D * 2;
-  static constexpr int T_BYTES = KN * D * 2;
+  static constexpr int T_BYTES = KB * KN * 128;
   static constexpr int OFF_RING = Q_BYTES;
   static constexpr int OFF_RAW = OFF_RING + RING * T_BYTES;
   static constexpr int OFF_FACTOR = OFF_RAW + (Q8 ? CVT_WARPS * RAW * RAW_BYTES : 0);  // [QM] softmax factors
