@@ -706,18 +706,24 @@ __global__ void __launch_bounds__(128) k_attn_join(const DecodeAttnArgs a, int r
 
 // How a call is cut. (tiles: false for what the tcgen05 kernel cannot describe,
 // which then needs no workspace either.)
-//  - Items of more than kFewRows rows: tiles of 128 rows on tcgen05
+//  - Items of many rows (few_rows below): tiles of 128 rows on tcgen05
 //    (decode_attn_tc.cu), the keys in parts where there are few tiles.
 //  - Blocks of 8 rows, or of 16 where an item has more: they share one read of
 //    the keys.
-//  - Twelve warps run on an SM. Many blocks: a warp takes one alone (CTAs of
-//    one warp, no join); fewer: four warps share one.
+//  - Eight to 16 warps run on an SM, by their registers. Many blocks: a warp
+//    takes one alone (CTAs of one warp, no join); fewer: four warps share one.
 //  - Still fewer: the keys are cut into parts of at least 128, one for each CTA
 //    of a cluster, which joins them: one launch and no workspace.
 //  - Where that leaves SMs without work and the parts are long, into more
 //    parts, about six CTAs an SM (lengths differ; three run at a time), joined
 //    by a second kernel.
-constexpr int kFewRows = 32;
+//  - Parts of less than 1024 keys, and one item's, which has one length: no more
+//    of them than run at a time, since a round of short ones is mostly their
+//    starts (64 sequences of 4 new tokens over 300, 16 heads of 64 for 4: one
+//    part 8 us, three 21; 16 clips of one row over 2000 keys, 8 heads of 128:
+//    three parts 24 us, six 28). Two that fill a little more than one round are
+//    kept down to 512 keys (32 clips of 4 rows over 200 to 1500, 8 heads of 64:
+//    18 us, one part 21).
 struct Plan {
   int rows, row_tiles, warps, n_split;  // warps 0: the tcgen05 kernel
   bool clustered;                       // the parts are joined in a cluster
@@ -754,10 +760,29 @@ int tile_parts(int n_items, long long blocks, int max_kv, bool q8) {
   return n < 1 ? 1 : (int)n;
 }
 
-Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, bool q8, bool tiles = true) {
+// Whether an item's rows for one key head are few, blocks of 16 of which read
+// the keys again, rather than a tile of 128 with its longer start:
+//  - up to 32;
+//  - up to 64 where the blocks have little to do, 2^22 keys x columns in all, or
+//    2^24 over the 8-bit cache, whose tiles cost more (one clip of 36 rows over
+//    500 keys, 8 heads of 64: 6 us, tiles 9; 4 clips over 1500: 16 and 14 us.
+//    16 new tokens of 32 heads for 8 of 128 over 4000 cached ones: 15 us, tiles
+//    21; over 60000: 107 and 89 us);
+//  - over at most 2048 cached tokens up to 48, or 64 of 64 columns (128
+//    sequences of 100 to 1500, 36 to 64 rows of 64 columns: 54 to 67 us, tiles
+//    87 to 90; 200 of 36 rows of 128 columns 85 and 120 us).
+bool few_rows(long long rows, int n_items, int max_kv, int n_kv_heads, int head_dim, bool q8) {
+  if (rows <= 32) return true;
+  if (rows > 64) return false;
+  const double work = (double)n_items * n_kv_heads * ((rows + 15) / 16) * max_kv * head_dim;
+  return work <= (q8 ? 1 << 24 : 1 << 22) || (q8 && max_kv <= 2048 && (rows <= 48 || head_dim == 64));
+}
+
+Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, int head_dim, bool q8,
+               bool tiles_ok = true) {
   Plan p;
   const long long rows = (long long)max_q * (n_heads / n_kv_heads);
-  if (rows > kFewRows && tiles) {
+  if (tiles_ok && !few_rows(rows, n_items, max_kv, n_kv_heads, head_dim, q8)) {
     p.rows = kTileRows;
     p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
     p.blocks = (long long)n_items * n_kv_heads * p.row_tiles;
@@ -769,15 +794,21 @@ Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, 
   p.rows = rows <= 8 ? 8 : 16;
   p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
   p.blocks = (long long)n_items * n_kv_heads * p.row_tiles;
-  constexpr long long slots = 12LL * kSms;
-  p.warps = 2 * p.blocks > slots ? 1 : 4;
+  // warps that run at a time; rounds of CTAs of w warps over tiles of keys, the
+  // start and the end of a CTA counted as five tiles
+  const int warps_sm = head_dim == 128 ? (p.rows == 8 ? 12 : 8) : p.rows == 8 ? 16 : q8 ? 8 : 12;
+  const long long slots = (long long)warps_sm * kSms, tiles = max_kv / (q8 ? 32 : 16) + 1;
+  auto cost = [&](int w) { return (p.blocks * w + slots - 1) / slots * ((tiles + w - 1) / w + 5); };
+  p.warps = p.blocks > 6 * kSms || (4 * p.blocks > slots && cost(1) < cost(4)) ? 1 : 4;
   p.n_split = 1;
   p.clustered = false;
-  if (p.warps == 4 && tiles && p.blocks > 0) {
-    const long long most = ((long long)max_kv + 127) / 128, want = 2 * slots / (4 * p.blocks);  // two rounds of CTAs
+  if (p.warps == 4 && tiles_ok && p.blocks > 0) {
+    const long long most = ((long long)max_kv + 127) / 128, want = 6LL * kSms / p.blocks, round = slots / 4 / p.blocks;
     const long long n0 = want < most ? want : most;
     p.clustered = n0 <= 8 || max_kv <= 8 * 1024;
-    const long long n = p.clustered && n0 > 8 ? 8 : n0 > 64 ? 64 : n0;
+    long long n = p.clustered && n0 > 8 ? 8 : n0 > 64 ? 64 : n0;
+    const bool brief = max_kv < 1024 * n && (round > 1 || max_kv < 512 * n);
+    if ((n_items == 1 || brief) && n > round) n = round;
     p.n_split = n < 1 ? 1 : (int)n;
     p.clustered = p.clustered && p.n_split > 1;
   }
@@ -817,7 +848,7 @@ cudaError_t launch_w(const DecodeAttnArgs& a, const Plan& p, cudaStream_t st) {
 
 template <typename H, bool Q8, int D, int WT>
 cudaError_t launch_rows(const DecodeAttnArgs& a, cudaStream_t st) {
-  const Plan p = plan_rows(a.n_items, a.max_q, a.max_kv, a.n_heads, a.n_kv_heads, Q8, attn_tiles_fit(a));
+  const Plan p = plan_rows(a.n_items, a.max_q, a.max_kv, a.n_heads, a.n_kv_heads, D, Q8, attn_tiles_fit(a));
   if (p.blocks * p.n_split * p.rows > 0x7fffffffLL) return cudaErrorInvalidValue;
   if (p.warps == 0) {
     const cudaError_t e = attn_tiles_launch(a, is_bf16<H>::value, p.row_tiles, p.n_split, st);
@@ -843,7 +874,7 @@ cudaError_t launch_h(const DecodeAttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 size_t decode_attn_ws_bytes(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, int head_dim, bool q8) {
-  const Plan p = plan_rows(n_items, max_q, max_kv, n_heads, n_kv_heads, q8);
+  const Plan p = plan_rows(n_items, max_q, max_kv, n_heads, n_kv_heads, head_dim, q8);
   return p.n_split == 1 || p.clustered ? 0 : (size_t)p.blocks * p.n_split * p.rows * (head_dim + 2) * sizeof(float);
 }
 
