@@ -35,10 +35,11 @@
 // of shared memory, 48 cycles, for 32 of products), and about 10,000 cycles a
 // CTA lie before its first and behind its last tile. 8 x 100 to 256 new tokens
 // over 300 to 16384 cached ones, 16 heads of 64 for 4, pages of 64: 174 us, 300
-// TFLOP/s: a tile takes 3000 cycles, in which conversion and softmax share the
-// issue slots and the registers (96). Two row tiles a CTA under one conversion
-// took 186 us (16-bit keys: 135 instead of 104), three converting warps and 128
-// registers 169 us but up to 19% more with 128 columns.
+// TFLOP/s: a tile takes a CTA 2400 cycles and more, of which its softmax warps
+// work 1860 (96 registers, beside converting warps that use a third of the issue
+// slots) and wait the rest; 53% of the issue slots are used. Two row tiles a CTA
+// under one conversion took 186 us (16-bit keys: 135 instead of 104), three
+// converting warps and 128 registers 169 us but up to 19% more with 128 columns.
 #include "common.cuh"
 #include "decode.h"
 #include "decode_common.cuh"
