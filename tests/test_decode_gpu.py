@@ -114,6 +114,16 @@ def test_cross_attention(cuda, bf16, q_lens, kv_lens, H, Hkv, D):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("q_lens,kv_lens,H,Hkv,D", [
+    ([36], [500], 8, 8, 64), ([64, 0, 50], [200, 9, 0], 4, 4, 128), ([12, 11, 9] * 14, [7, 130, 64] * 14, 4, 1, 64),
+    ([16, 15], [390, 17], 4, 1, 128), ([150], [3001], 2, 1, 128), ([9, 70, 1], [2500, 300, 1100], 3, 3, 64),
+])
+def test_cross_attention_between_few_and_many_rows(cuda, bf16, q_lens, kv_lens, H, Hkv, D):
+    """33 to 64 rows (blocks of 16, or a tile), and parts of one item's keys."""
+    check_cross(cuda, q_lens, kv_lens, H, Hkv, D, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("n", [1, 200])
 def test_cross_attention_long_and_peaked(cuda, bf16, n):
     """Many keys, and scores so far apart that one key has nearly all weight."""
@@ -480,6 +490,17 @@ KV8 = [
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("q_lens,lens,H,Hkv,D,page", KV8)
 def test_kv8_attention(cuda, bf16, q_lens, lens, H, Hkv, D, page):
+    check_kv8(cuda, q_lens, lens, H, Hkv, D, page, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("q_lens,lens,H,Hkv,D,page", [
+    ([16], [500], 16, 4, 128, 64), ([16, 5, 1], [333, 70, 1], 8, 2, 64, 16), ([12, 9] * 35, [163, 40] * 35, 16, 4, 64, 32),
+    ([9, 12, 8], [1500, 2048, 700], 16, 4, 128, 128), ([12, 3], [3000, 999], 16, 4, 128, 32), ([256], [5000], 4, 1, 64, 64),
+    ([16, 2], [2500, 129], 16, 4, 64, 16),
+])
+def test_kv8_attention_between_few_and_many_rows(cuda, bf16, q_lens, lens, H, Hkv, D, page):
+    """33 to 64 rows (blocks of 16, or a tile), and parts of one sequence's tokens."""
     check_kv8(cuda, q_lens, lens, H, Hkv, D, page, bf16)
 
 
