@@ -458,7 +458,9 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
       }
       if constexpr (Q8) ref = ti.z;
     }
-    if (ok) ok = o_settled();
+    // (without a tile nothing above has waited for the other warps' rows of Q,
+    // which lie where this one's output goes)
+    if (ok) ok = nT > 0 ? o_settled() : wwait(B_QREADY, 0);
     // ---- O / l, through this warp's rows of the Q tile (every product that
     // reads Q is done), stored as whole rows; or the part's sums
     if (ok) {

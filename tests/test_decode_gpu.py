@@ -131,6 +131,14 @@ def test_cross_attention_long_and_peaked(cuda, bf16, n):
     check_cross(cuda, [n, 3], [700, 90], 4, 2, 128, bf16, q_scale=20.0)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_cross_attention_many_rows_without_keys(cuda, D):
+    """Tiles of rows that have no key give zeros, all of them."""
+    for seed in range(3):
+        check_cross(cuda, [88, 68, 14, 112, 76, 25, 128, 130, 70] * 9, [2, 0, 0, 0, 2, 0, 0, 0, 0] * 9, 4, 4, D, False,
+                    seed=seed)
+
+
 @pytest.mark.parametrize("n", [2, 150])
 def test_cross_attention_max_q_above_the_rows(cuda, n):
     """max_q is a bound: a larger one changes nothing."""
