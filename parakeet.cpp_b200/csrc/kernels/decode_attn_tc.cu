@@ -28,6 +28,10 @@
 // moves to the tile's largest scale and O is multiplied. A tile of several
 // small pages that are further apart than that takes them one after another,
 // each under its own reference (16 keys of one product step lie in one page).
+// A page more than 2^80 below the largest one so far (all zeros, as a rule:
+// their scale is 2^-126) counts as zeros and moves nothing. So O stays finite
+// however far ref falls: with weights up to 2^8, 2^30 keys and codes up to 448 it
+// is below 2^47 in units of the largest scale, and below 2^127 in those of ref.
 //
 // Measured: 64 x 130 to 384 rows over 250 to 1500 keys, 8 heads of 128: 104 us,
 // 570 TFLOP/s. A tile takes a CTA 1450 cycles beside the other CTA's; the
@@ -110,9 +114,11 @@ __device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
   return r;
 }
 
-__device__ __forceinline__ float pow2i(int e) {
-  e = e < -126 ? -126 : e > 127 ? 127 : e;
-  return __int_as_float((e + 127) << 23);
+constexpr int kFarBelow = 80;  // exponents; see above
+constexpr int kNoPage = -1000;
+
+__device__ __forceinline__ float pow2i(int e) {  // 2^e for e <= 127; 0 below 2^-126
+  return e < -126 ? 0.f : __int_as_float((e + 127) << 23);
 }
 
 template <typename H, bool Q8, int D>
@@ -589,7 +595,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
         cp_commit();
       };
       const int c0 = (2 * ch) & 7, flip = (ch >> 2) & 1;
-      int ref = 0;
+      int ref = 0, most = kNoPage;  // the reference, the largest exponent of a page so far
       bool ok = true;
       int id_next = page_id(0);
 #pragma unroll
@@ -623,23 +629,39 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
           int parts = 1;
           if (one) {
             if (none) {  // no values
-            } else if (t > 0 && ev - ref <= 7 && ev - ref >= -15) {
-              dv = ev - ref;
+            } else if (most - ev > kFarBelow) {
+              dv = kNoPage;  // its values times 0
             } else {
-              grow = t > 0 ? pow2i(ref - ev) : 1.f;
-              ref = ev;
+              if (most != kNoPage && ev - ref <= 7 && ev - ref >= -15) {
+                dv = ev - ref;
+              } else {
+                grow = most != kNoPage ? pow2i(ref - ev) : 1.f;
+                ref = ev;
+              }
+              most = max(most, ev);
             }
           } else {
-            const bool counts = in && !none;
-            const int mx = __reduce_max_sync(0xffffffffu, counts ? ev : -1000);
+            // the largest exponent of the pages before lane j's
+            int before_j = in && !none ? ev : kNoPage;
+#pragma unroll
+            for (int k = 1; k < KN / 16; k <<= 1) {
+              const int y = __shfl_up_sync(0xffffffffu, before_j, k);
+              if (lane >= k) before_j = max(before_j, y);
+            }
+            before_j = __shfl_up_sync(0xffffffffu, before_j, 1);
+            before_j = lane == 0 ? most : max(before_j, most);
+            const bool far = in && !none && before_j - ev > kFarBelow;
+            const bool counts = in && !none && !far;
+            const int mx = __reduce_max_sync(0xffffffffu, counts ? ev : kNoPage);
             const int mn = __reduce_min_sync(0xffffffffu, counts ? ev : 1000);
-            if (mx == -1000) {  // no values
-            } else if (t > 0 && mx - ref <= 7 && mn - ref >= -15) {
-              dv = counts ? ev - ref : 0;  // (0: no values there)
+            if (far) dv = kNoPage;
+            if (mx == kNoPage) {  // no values
+            } else if (most != kNoPage && mx - ref <= 7 && mn - ref >= -15) {
+              if (counts) dv = ev - ref;
             } else if (mx - mn <= 15) {
-              grow = t > 0 ? pow2i(ref - mx) : 1.f;
+              grow = most != kNoPage ? pow2i(ref - mx) : 1.f;
               ref = mx;
-              dv = counts ? ev - ref : 0;
+              if (counts) dv = ev - ref;
             } else {
               // each counting page under its own reference; from which one O
               // comes to it: the last counting page before, or the tile before
@@ -648,9 +670,10 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
               const uint32_t before = have & ((1u << lane) - 1u);
               const int last = 31 - __clz(have);
               const int prev = __shfl_sync(0xffffffffu, ev, before ? 31 - __clz(before) : 0);
-              grow = !counts ? 1.f : before ? pow2i(prev - ev) : t > 0 ? pow2i(ref - ev) : 1.f;
+              grow = !counts ? 1.f : before ? pow2i(prev - ev) : most != kNoPage ? pow2i(ref - ev) : 1.f;
               ref = __shfl_sync(0xffffffffu, ev, last);
             }
+            most = max(most, mx);
           }
           if (w == CVT_WARPS / 2) {
             // (info t - RING was read before P V of t - 3, which had to be done
