@@ -145,7 +145,6 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
   const int h = rest % a.n_kv_heads, b = rest / a.n_kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
-  pdl_trigger();
   const Item it = load_item<Q8>(a, b);
   if (!it.ok) {
     if (threadIdx.x == 0) report_error(a.err, DEV_ERR_BAD_SHAPE);
@@ -224,6 +223,9 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // (not before this block has its tensor memory: a dependent kernel's block
+  // may take all of the SM's and then wait for this kernel's end)
+  pdl_trigger();
   const uint32_t tmem = *tmem_slot;
   auto wwait = [&](int i, uint32_t parity) -> bool {
     return __all_sync(0xffffffffu, mbar_wait(bar(i), parity, a.err, DEV_ERR_TIMEOUT_ATTN)) != 0;
