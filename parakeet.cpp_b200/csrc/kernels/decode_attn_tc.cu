@@ -474,7 +474,8 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
     if (ok) {
       const float back = Q8 && nT > 0 ? pow2i((int)ref) : 1.f;
       if (n_split == 1) {
-        const float inv = lsum == 0.f ? 0.f : back / lsum;  // no key seen: zeros
+        // (1 / l and 2^ref apart: their product may be too small for all of its bits)
+        const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // no key seen: zeros
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -487,7 +488,8 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              w[e] = lsum == 0.f ? 0u : pack2<H>(__uint_as_float(o[8 * k + 2 * e]) * inv, __uint_as_float(o[8 * k + 2 * e + 1]) * inv);
+              w[e] = lsum == 0.f ? 0u : pack2<H>(__uint_as_float(o[8 * k + 2 * e]) * inv * back,
+                                                 __uint_as_float(o[8 * k + 2 * e + 1]) * inv * back);
             *reinterpret_cast<uint4*>(sm + i * (D * 2) + (((4 * c + k) ^ (i & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }

@@ -1,0 +1,39 @@
+"""The attention decoder's operators at the ends of their types' ranges and
+where a call is partly wrong."""
+import pytest
+
+from test_decode_gpu import make_cache, run_kv8
+
+pytestmark = pytest.mark.gpu
+
+
+def test_kv8_attention_tiny_values_long_sums(cuda):
+    """Values at the smallest scale (2^-126) under equal weights of 60,000 keys:
+    the mean keeps its precision. Codes are multiples of 8 up to 120, so sums
+    are whole numbers below 2^24 and exact; what is left is a reciprocal, two
+    products and the output's rounding (bf16 keeps 8 bits: half a step is 2^-8
+    of the value at most)."""
+    import torch
+    page, D, H, n, t = 128, 64, 32, 1184, 65000
+    c = make_cache(cuda, 1, [t], 1, D, page)
+    g = torch.Generator(device=cuda).manual_seed(5)
+    code = (torch.randint(8, 16, c["v"].shape, generator=g, device=cuda) * 8).float()
+    c["v"].copy_(code.to(torch.float8_e4m3fn).view(torch.uint8))
+    c["k"].zero_()
+    c["k_scale"].fill_(1.0)
+    c["v_scale"].fill_(2.0 ** -126)
+    # two sequences of the same pages: as many rows as leave the keys in one part
+    c["table"] = c["table"].repeat(2, 1).contiguous()
+    c["c"].table = c["table"].data_ptr()
+    q = torch.randn(2 * n, H * D, generator=g, device=cuda).bfloat16()
+    out = torch.full((2 * n, H * D), -7.0, dtype=torch.bfloat16, device=cuda)
+    import pkc
+    assert pkc.kv8_attention_workspace(c["c"], 2, n, t, H) == 0
+    run_kv8(c, q, [n, n], [t, t], H, out)
+    assert int(c["err"]) == 0
+    v = code[c["table"][0, : -(-t // page)].long()].double().reshape(-1, D)[:t]
+    sees = torch.arange(t - n + 1, t + 1, device=cuda)
+    mean = v.cumsum(0)[sees - 1] / sees[:, None] * 2.0 ** -126
+    tol = mean * (2.0 ** -8 + 8 * 2.0 ** -24)
+    got = out.double().view(2, n, H, D)
+    assert ((got - mean[None, :, None]).abs() <= tol[None, :, None]).all()
