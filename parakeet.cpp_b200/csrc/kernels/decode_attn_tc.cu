@@ -70,10 +70,10 @@ enum : int {
 
 // What the converting warps tell the softmax about a tile.
 struct TileInfo {
-  float4 head;    // key scale (of a tile in one page; negative: a page that is none), what O is multiplied by
-                  // before the tile is added, the exponent that O is kept under behind the tile, parts (1, or the
-                  // tile's pages)
-  float4 ks;      // several pages: key scale of each 16 keys
+  float4 head;    // the largest key scale (of a tile in one page: its own, negative: a page that is none), what O is
+                  // multiplied by before the tile is added, the exponent that O is kept under behind the tile,
+                  // parts (1, or the tile's pages)
+  float4 ks;      // several pages: key scale of each 16 keys over the largest; negative: a page that is none
   float grow[4];  // and, where it has parts, what O is multiplied by before each
 };
 
@@ -341,7 +341,9 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(B_QREADY));
 
-    const float rs = fmaxf(s_factor[i], kTiny);
+    // (over the 8-bit cache together with a key scale: the one may be as small
+    // as the other is large)
+    const float rs = Q8 ? s_factor[i] : fmaxf(s_factor[i], kTiny);
     const int vis = i < valid ? visible<Q8>(it, (row0 + i) / G) : 0;
     float m_used = -INFINITY, lsum = 0.f, ref = 0.f;
     bool ok = true;
@@ -391,9 +393,8 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
       }
       float c = rs;
       if constexpr (Q8) {
-        if (np == 1) {
-          c = fmaxf(c * fabsf(ti.x), kTiny);
-        } else {
+        c = fmaxf(c * fabsf(ti.x), kTiny);
+        if (np > 1) {
 #pragma unroll
           for (int j = 0; j < KN; ++j) x[j] *= fabsf(j < 16 ? ks4.x : j < 32 ? ks4.y : j < 48 ? ks4.z : ks4.w);
         }
@@ -683,18 +684,22 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
             // (info t - RING was read before P V of t - 3, which had to be done
             // for the place of values t - 1, or of keys t - 1 before it)
             TileInfo* ti = info(t);
+            float ks_most = ks;
             if (!one) {
               const int j = lane < 4 ? (lane * 16) >> shift : 0;
-              const float ks_j = __shfl_sync(0xffffffffu, ks, j);
-              const bool in_j = __shfl_sync(0xffffffffu, (int)in, j);
+              const int ek = ((__float_as_int(ks) >> 23) & 255) - 127;
+              const int ek_most = __reduce_max_sync(0xffffffffu, in && !none ? ek : kNoPage);
+              const float over = none ? -1.f : in ? pow2i(ek - ek_most) : 1.f;  // (keys behind the last are masked)
+              const float over_j = __shfl_sync(0xffffffffu, over, j);
               if (lane < 4) {
-                reinterpret_cast<float*>(&ti->ks)[lane] = in_j ? ks_j : 1.f;  // (keys behind the last are masked)
+                reinterpret_cast<float*>(&ti->ks)[lane] = over_j;
                 ti->grow[lane] = grow;
               }
+              ks_most = ek_most == kNoPage ? 1.f : pow2i(ek_most);
               __syncwarp();
             }
             if (lane == 0) {
-              ti->head = make_float4(ks, grow, (float)ref, (float)parts);
+              ti->head = make_float4(ks_most, grow, (float)ref, (float)parts);
               mbar_arrive(bar(B_INFO + t % RING));
             }
           }

@@ -2,7 +2,7 @@
 where a call is partly wrong."""
 import pytest
 
-from test_decode_gpu import make_cache, run_kv8
+from test_decode_gpu import append, make_cache, run_kv8, values
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,30 @@ def test_kv8_attention_tiny_values_long_sums(cuda):
     tol = mean * (2.0 ** -8 + 8 * 2.0 ** -24)
     got = out.double().view(2, n, H, D)
     assert ((got - mean[None, :, None]).abs() <= tol[None, :, None]).all()
+
+
+@pytest.mark.parametrize("n", [1, 20, 140])
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("e", [124, -124])
+def test_kv8_attention_ordinary_scores_of_extreme_keys(cuda, n, page, e):
+    """bf16 keys about 2^124 with queries about 2^-124, and the other way
+    round: neither's size alone may leave f32."""
+    import decode_ref
+    import torch
+    g = torch.Generator().manual_seed(page + n)
+    t, D = 300, 64
+    new = torch.randn(t, 2, 1, D, generator=g)
+    new[:, 0] *= 2.0 ** e
+    new = new.bfloat16().to(cuda)
+    c = make_cache(cuda, 1, [t], 1, D, page)
+    append(c, new, [t], [t])
+    ids = c["table"][0, : -(-t // page)].long()
+    k, v = ((values(c, x)[ids] * c[x + "_scale"][ids].double()[..., None, None]).transpose(1, 2).reshape(-1, 1, D)[:t] for x in "kv")
+    q = (torch.randn(n, D, generator=g) * 2.0 ** -e).bfloat16().to(cuda)
+    out = torch.full((n, D), -7.0, dtype=torch.bfloat16, device=cuda)
+    run_kv8(c, q, [n], [t], 1, out)
+    assert int(c["err"]) == 0
+    o, A, S = decode_ref.attention(q.double().view(n, 1, D), k, v, D ** -0.5, True)
+    tol = decode_ref.attention_tolerance(o, A, S, float(v.abs().max()), t, D, torch.bfloat16, torch.float16)
+    got = out.double().view(n, 1, D)
+    assert torch.isfinite(got).all() and ((got - o).abs() <= tol).all()
