@@ -494,8 +494,8 @@ pkc_status pkc_kv8_reorder(const pkc_kv8_cache* cache, const int* parent, const 
    scores are formed in f64 and rounded once), finished [B, K] uint8 or NULL: a
    finished hypothesis offers itself alone, with token eos and its score.
    parent, token [B, K] int32; finished_out [B, K] (or NULL): token is eos, or
-   the parent had finished. A row with a NaN or +inf, or all -inf, and a NaN in
-   cum offer -inf. score may be cum, finished_out may be finished; logits row
+   the parent had finished. A row with a NaN or +inf, or all -inf, and a cum that
+   is not finite offer -inf. score may be cum, finished_out may be finished; logits row
    stride ld. At the first step give hypotheses 1 .. K-1 a cum of -inf. */
 pkc_status pkc_beam_select(const void* logits, long long ld, int dtype, const float* cum, const uint8_t* finished,
                            int B, int K, int V, int eos, float* score, int* parent, int* token, uint8_t* finished_out,

@@ -5,8 +5,8 @@
 // each: score(beam, v) = cum[beam] + x_v - log sum_u exp(x_u). The K best of
 // the K * V continuations are taken, ties to the lowest beam * V + v. A
 // finished hypothesis offers itself alone (its end token, score unchanged); a
-// row whose sum is not finite (NaN, +inf, or nothing but -inf) and a score
-// that is NaN offer -inf.
+// row whose sum is not finite (NaN, +inf, or nothing but -inf) and a
+// hypothesis whose score is not finite offer -inf.
 //
 // Within a row the order is that of the logits, so each CTA reads its row (or
 // its part of one) once from memory and keeps the K largest as keys (ordered
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_select(const BeamSelectArg
   const bool fin = on && a.finished && a.finished[(long long)b * K + beam];
   // 0: a live row; 1: finished, its end token, then the lowest others; 2: one
   // that offers nothing, its lowest tokens
-  const int kind = cum != cum || cum == -INFINITY ? 2 : fin ? 1 : s > 0.0 && isfinite(s) && isfinite(m) ? 0 : 2;
+  const int kind = !isfinite(cum) ? 2 : fin ? 1 : s > 0.0 && isfinite(s) && isfinite(m) ? 0 : 2;
   const double lse = (double)m + log(s);
   const Part& mine = sh.part[on ? lane : 0];
   const bool lists = on && (kind == 0 || lane % chunks == 0);

@@ -2,7 +2,7 @@
 where a call is partly wrong."""
 import pytest
 
-from test_decode_gpu import append, make_cache, run_kv8, values
+from test_decode_gpu import append, make_cache, run_kv8, run_select, values
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,31 @@ def test_kv8_attention_ordinary_scores_of_extreme_keys(cuda, n, page, e):
     tol = decode_ref.attention_tolerance(o, A, S, float(v.abs().max()), t, D, torch.bfloat16, torch.float16)
     got = out.double().view(n, 1, D)
     assert torch.isfinite(got).all() and ((got - o).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("V", [60, 9000])
+def test_beam_select_infinite_scores(cuda, V):
+    """A score of +inf offers -inf like one that is not a number, whether its
+    row has masked tokens, has finished or neither."""
+    import decode_ref
+    import torch
+    B, K = 4, 4
+    g = torch.Generator().manual_seed(V)
+    logits = torch.randn(B, K, V, generator=g).to(cuda)
+    cum = torch.randn(B, K, generator=g).to(cuda)
+    fin = torch.zeros(B, K, dtype=torch.uint8, device=cuda)
+    cum[0, 1] = float("inf")
+    cum[1, 2] = float("inf")
+    logits[1, 2, 3:] = float("-inf")
+    cum[2, 0] = float("inf")
+    fin[2, 0] = 1
+    cum[3] = float("inf")
+    score, parent, token, done = run_select(logits, cum, fin, V - 1)
+    dead = torch.where(cum == float("inf"), float("-inf"), cum)
+    rs, rp, rt, rd = decode_ref.beam_select(logits, dead, fin.bool(), V - 1)
+    assert not torch.isnan(score).any()
+    assert torch.equal(parent.long(), rp) and torch.equal(token.long(), rt) and torch.equal(done.bool(), rd)
+    live = torch.isfinite(rs)
+    assert torch.equal(torch.isfinite(score), live) and (score[~live] == float("-inf")).all()
+    # exponentials within 2^-22 of their values, so is their sum's logarithm; one rounding to f32
+    assert ((score.double() - rs)[live].abs() <= 2.0 ** -21 + rs[live].abs() * 2.0 ** -24 * 1.01).all()
