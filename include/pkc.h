@@ -413,7 +413,7 @@ pkc_status pkc_relpos_attention_noalloc(const void* qkv, const void* ptab, int c
 
    What only the device knows is checked there: an offset, length, page or
    parent outside the sizes that the call was given leaves that item (for a
-   page: its tokens) out, and the first such error's code goes to *err, a
+   page its tokens, for a parent of pkc_beam_reorder its row) out, and the first such error's code goes to *err, a
    device int that the caller zeroes and reads when it likes (110: out of the
    sizes, 111: a value that is not a number); err may be NULL. Rows that
    belong to no item are left as they were.
@@ -505,7 +505,8 @@ pkc_status pkc_beam_select(const void* logits, long long ld, int dtype, const fl
    blocks becomes a copy of what row b*K + parent[b*K + k] was. Rows are
    row_bytes long, row_stride bytes apart, blocks outer_stride bytes (any
    alignment; 16 is fastest). lens (or NULL): only the first
-   lens[b] * unit_bytes of a row are live. K <= 32. */
+   lens[b] * unit_bytes of a row are live. A bad parent leaves its row as it
+   was, a negative length its item; both are reported. K <= 32. */
 pkc_status pkc_beam_reorder(void* state, const int* parent, int B, int K, long long row_bytes, long long row_stride,
                             int n_outer, long long outer_stride, const int* lens, long long unit_bytes, int* err,
                             void* stream);

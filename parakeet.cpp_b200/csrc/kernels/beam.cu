@@ -409,7 +409,9 @@ __global__ void __launch_bounds__(256, KM <= 8 ? 4 : KM <= 16 ? 2 : 1) k_beam_re
   __syncthreads();
   long long bytes = a.row_bytes;
   if (a.lens) {
-    const long long live = a.lens[b] > 0 ? a.lens[b] * a.unit_bytes : 0;
+    const int len = a.lens[b];
+    if (len < 0 && threadIdx.x == 0) report_error(a.err, DEV_ERR_BAD_SHAPE);
+    const long long live = len > 0 ? len * a.unit_bytes : 0;
     bytes = live < bytes ? live : bytes;
   }
   const long long cols = bytes / (long long)sizeof(V), tail = bytes % (long long)sizeof(V);

@@ -2,7 +2,7 @@
 where a call is partly wrong."""
 import pytest
 
-from test_decode_gpu import append, make_cache, run_kv8, run_select, values
+from test_decode_gpu import append, make_cache, run_kv8, run_select, stream, values
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,23 @@ def test_beam_select_infinite_scores(cuda, V):
     assert torch.equal(torch.isfinite(score), live) and (score[~live] == float("-inf")).all()
     # exponentials within 2^-22 of their values, so is their sum's logarithm; one rounding to f32
     assert ((score.double() - rs)[live].abs() <= 2.0 ** -21 + rs[live].abs() * 2.0 ** -24 * 1.01).all()
+
+
+def test_beam_reorder_negative_length_is_reported(cuda):
+    """A negative length leaves its item as it is and is reported; the other
+    items move. A length of zero is no error."""
+    import pkc
+    import torch
+    for bad in (-1, 0):
+        x = torch.arange(12, dtype=torch.float32, device=cuda).view(3, 4, 1).repeat(1, 1, 8).clone()
+        before = x.clone()
+        err = torch.zeros(1, dtype=torch.int32, device=cuda)
+        parent = torch.tensor([[3, 2, 1, 0]] * 3, dtype=torch.int32, device=cuda)
+        lens = torch.tensor([2, bad, 2], dtype=torch.int32, device=cuda)
+        pkc.beam_reorder(x.data_ptr(), parent.data_ptr(), 3, 4, row_bytes=32, lens=lens.data_ptr(), unit_bytes=16,
+                         err=err.data_ptr(), stream=stream())
+        torch.cuda.synchronize()
+        assert int(err) == (110 if bad < 0 else 0)
+        assert torch.equal(x[1], before[1])
+        for b in (0, 2):
+            assert torch.equal(x[b], before[b].flip(0))
