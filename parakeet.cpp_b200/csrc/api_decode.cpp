@@ -269,7 +269,8 @@ extern "C" pkc_status pkc_beam_reorder(void* state, const int* parent, int B, in
       return bad(what, "B and n_outer must be in [0, 65535] and K in [1, 32]");
     if (row_bytes < 0 || row_stride < row_bytes || (lens && (unit_bytes < 0 || unit_bytes > (1LL << 31))))
       return bad(what, "bad row_bytes, row_stride or unit_bytes");
-    if (n_outer > 1 && outer_stride < (long long)B * K * row_stride)
+    // (a quotient: the product may pass 64 bits)
+    if (n_outer > 1 && B > 0 && outer_stride / ((long long)B * K) < row_stride)
       return bad(what, "blocks overlap: outer_stride is less than B * K * row_stride");
     if (B == 0 || n_outer == 0 || row_bytes == 0) return PKC_OK;
     if (!state || !parent) return bad(what, "a pointer is NULL");
