@@ -725,10 +725,16 @@ __global__ void __launch_bounds__(128) k_attn_join(const DecodeAttnArgs a, int r
 //    kept down to 512 keys (32 clips of 4 rows over 200 to 1500, 8 heads of 64:
 //    18 us, one part 21).
 struct Plan {
-  int rows, row_tiles, warps, n_split;  // warps 0: the tcgen05 kernel
-  bool clustered;                       // the parts are joined in a cluster
-  long long blocks;
+  int rows, warps, n_split;  // warps 0: the tcgen05 kernel
+  bool clustered;            // the parts are joined in a cluster
+  long long row_tiles, blocks;
 };
+// Blocks of a call whose bounds may be loose; more than a grid has count as
+// 2^31, which is refused where the call is launched.
+long long count_blocks(int n_items, int n_kv_heads, long long row_tiles) {
+  const double n = (double)n_items * n_kv_heads * (double)row_tiles;
+  return n < (double)(1LL << 31) ? (long long)n_items * n_kv_heads * row_tiles : 1LL << 31;
+}
 // Parts of the keys for the tcgen05 kernel, of at least 256 keys; 2 * kSms CTAs
 // run at a time.
 //  - One item: the number that ends first, in tiles one after another, the start
@@ -784,16 +790,16 @@ Plan plan_rows(int n_items, int max_q, int max_kv, int n_heads, int n_kv_heads, 
   const long long rows = (long long)max_q * (n_heads / n_kv_heads);
   if (tiles_ok && !few_rows(rows, n_items, max_kv, n_kv_heads, head_dim, q8)) {
     p.rows = kTileRows;
-    p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
-    p.blocks = (long long)n_items * n_kv_heads * p.row_tiles;
+    p.row_tiles = (rows + p.rows - 1) / p.rows;
+    p.blocks = count_blocks(n_items, n_kv_heads, p.row_tiles);
     p.warps = 0;
     p.clustered = false;
     p.n_split = tile_parts(n_items, p.blocks, max_kv, q8);
     return p;
   }
   p.rows = rows <= 8 ? 8 : 16;
-  p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
-  p.blocks = (long long)n_items * n_kv_heads * p.row_tiles;
+  p.row_tiles = (rows + p.rows - 1) / p.rows;
+  p.blocks = count_blocks(n_items, n_kv_heads, p.row_tiles);
   // warps that run at a time; rounds of CTAs of w warps over tiles of keys, the
   // start and the end of a CTA counted as five tiles
   const int warps_sm = head_dim == 128 ? (p.rows == 8 ? 12 : 8) : p.rows == 8 ? 16 : q8 ? 8 : 12;
@@ -840,10 +846,10 @@ cudaError_t launch_w(const DecodeAttnArgs& a, const Plan& p, cudaStream_t st) {
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = p.clustered ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, a, p.row_tiles, p.n_split, p.clustered ? 1 : 0);
+  e = cudaLaunchKernelEx(&cfg, kern, a, (int)p.row_tiles, p.n_split, p.clustered ? 1 : 0);
   if (e != cudaSuccess || p.n_split == 1 || p.clustered) return e;
-  return launch_pdl(k_attn_join<H, Q8, D, 8 * NB, 4>, dim3((unsigned)(p.blocks * 8 * NB)), dim3(128), 0, st, a, p.row_tiles,
-                    p.n_split);
+  return launch_pdl(k_attn_join<H, Q8, D, 8 * NB, 4>, dim3((unsigned)(p.blocks * 8 * NB)), dim3(128), 0, st, a,
+                    (int)p.row_tiles, p.n_split);
 }
 
 template <typename H, bool Q8, int D, int WT>
@@ -851,10 +857,10 @@ cudaError_t launch_rows(const DecodeAttnArgs& a, cudaStream_t st) {
   const Plan p = plan_rows(a.n_items, a.max_q, a.max_kv, a.n_heads, a.n_kv_heads, D, Q8, attn_tiles_fit(a));
   if (p.blocks * p.n_split * p.rows > 0x7fffffffLL) return cudaErrorInvalidValue;
   if (p.warps == 0) {
-    const cudaError_t e = attn_tiles_launch(a, is_bf16<H>::value, p.row_tiles, p.n_split, st);
+    const cudaError_t e = attn_tiles_launch(a, is_bf16<H>::value, (int)p.row_tiles, p.n_split, st);
     if (e != cudaSuccess || p.n_split == 1) return e;
     return launch_pdl(k_attn_join<H, Q8, D, kTileRows, 1>, dim3((unsigned)(p.blocks * (kTileRows / 4))), dim3(128), 0, st, a,
-                      p.row_tiles, p.n_split);
+                      (int)p.row_tiles, p.n_split);
   }
   if (p.rows == 8)
     return p.warps == 1 ? launch_w<H, Q8, D, WT, 1, 1>(a, p, st) : launch_w<H, Q8, D, WT, 4, 1>(a, p, st);

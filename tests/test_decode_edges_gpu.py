@@ -2,7 +2,7 @@
 where a call is partly wrong."""
 import pytest
 
-from test_decode_gpu import append, make_cache, run_kv8, run_select, stream, values
+from test_decode_gpu import append, make_cache, offsets, run_kv8, run_select, stream, values
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +112,31 @@ def test_beam_reorder_negative_length_is_reported(cuda):
         assert torch.equal(x[1], before[1])
         for b in (0, 2):
             assert torch.equal(x[b], before[b].flip(0))
+
+
+def test_cross_attention_bound_beyond_a_grid_is_refused(cuda):
+    """A max_q so loose that its tiles pass a grid's size: an error, not a
+    wrapped number of tiles that leaves rows out. The largest that fits is
+    answered in full."""
+    import pkc
+    import torch
+    H, D, n = 512, 64, 2
+    q = torch.randn(n, H * D, device=cuda).half()
+    kv = torch.randn(9, 2, D, device=cuda).half()
+    out = torch.full_like(q, -7.0)
+    off, zero, nine = offsets([n], cuda), torch.zeros(1, dtype=torch.int32, device=cuda), torch.full((1,), 9, dtype=torch.int32, device=cuda)
+
+    def call(max_q):
+        pkc.cross_attention(q.data_ptr(), kv.data_ptr(), kv[:, 1].data_ptr(), off.data_ptr(), zero.data_ptr(), nine.data_ptr(), 1,
+                            H, 1, D, q_rows=n, kv_rows=9, max_q=max_q, max_kv=9, bf16=False, out=out.data_ptr(), ldk=2 * D,
+                            ldv=2 * D, stream=stream())
+        torch.cuda.synchronize()
+
+    with pytest.raises(pkc.PkcError):
+        call((1 << 30) + 1)  # 2^32 + 4 tiles of 128 rows
+    assert (out == -7).all()
+    call(2000)
+    s = torch.einsum("nhd,td->nht", q.double().view(n, H, D), kv[:, 0].double()) * D ** -0.5
+    ref = torch.einsum("nht,td->nhd", torch.softmax(s, -1), kv[:, 1].double()).flatten(1)
+    # weights and output are rounded to f16, half a step each
+    assert ((out.double() - ref).abs() <= float(kv.abs().max()) * 2.0 ** -10 + 2.0 ** -20).all()
