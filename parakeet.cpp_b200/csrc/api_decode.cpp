@@ -174,8 +174,11 @@ extern "C" pkc_status pkc_kv8_append(const pkc_kv8_cache* cache, const void* k, 
     const pkc_status ds = check_device(what, stream, {new_off, lens, cache->table, cache->k_scale, cache->v_scale, err},
                                        {k, v, cache->k, cache->v});
     if (ds != PKC_OK) return ds;
-    // (no sequence has more new tokens than there are)
-    pkc::Kv8AppendArgs a{kv8_of(cache), k, v, ldk, ldv, new_off, lens, n_seqs, rows, max_new < rows ? max_new : rows, err};
+    // (no sequence has more new tokens than there are, or than its pages hold)
+    const long long holds = (long long)cache->table_ld * cache->page;
+    int most = max_new < rows ? max_new : rows;
+    if (most > holds) most = (int)holds;
+    pkc::Kv8AppendArgs a{kv8_of(cache), k, v, ldk, ldv, new_off, lens, n_seqs, rows, most, err};
     return launched(what, pkc::kv8_append_launch(a, dtype == 1, reinterpret_cast<cudaStream_t>(stream)));
   });
 }

@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(256) k_kv8_reorder(const Kv8 c, const int* par
 
 template <typename H>
 cudaError_t append_h(const Kv8AppendArgs& a, cudaStream_t st) {
-  const int width = (a.max_new + a.c.page - 2) / a.c.page + 1;  // pages that a sequence's new tokens may touch
+  const int width = (int)(((long long)a.max_new + a.c.page - 2) / a.c.page) + 1;  // pages that a sequence's new tokens may touch
   const long long units = (long long)a.n_seqs * width * a.c.n_kv_heads * 2;
   if (units > 0x7fffffffLL) return cudaErrorInvalidValue;
   if (a.max_new <= 4)

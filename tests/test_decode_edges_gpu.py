@@ -140,3 +140,24 @@ def test_cross_attention_bound_beyond_a_grid_is_refused(cuda):
     ref = torch.einsum("nht,td->nhd", torch.softmax(s, -1), kv[:, 1].double()).flatten(1)
     # weights and output are rounded to f16, half a step each
     assert ((out.double() - ref).abs() <= float(kv.abs().max()) * 2.0 ** -10 + 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("bound", [(1 << 31) - 1, (1 << 31) - 15, 1 << 20])
+def test_kv8_append_loosest_bounds(cuda, bound):
+    """rows and max_new as loose as an int allows: every sequence is written as
+    with the true bounds."""
+    import pkc
+    import torch
+    Hkv, D, lens = 128, 64, [20, 33]
+    g = torch.Generator().manual_seed(1)
+    new = torch.randn(sum(lens), 2, Hkv, D, generator=g).half().to(cuda)
+    want, got = (make_cache(cuda, 2, lens, Hkv, D, 16) for _ in range(2))
+    append(want, new, lens, lens)
+    off, ln = offsets(lens, cuda), torch.tensor(lens, dtype=torch.int32, device=cuda)
+    pkc.kv8_append(got["c"], new.data_ptr(), new[:, 1].data_ptr(), off.data_ptr(), ln.data_ptr(), 2, rows=bound, max_new=bound,
+                   ldk=new.stride(0), ldv=new.stride(0), bf16=False, err=got["err"].data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    assert int(got["err"]) == 0
+    for x in "kv":
+        assert torch.equal(got[x], want[x])
+        assert torch.equal(got[x + "_scale"].nan_to_num(-1.0), want[x + "_scale"].nan_to_num(-1.0))
