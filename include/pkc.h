@@ -490,9 +490,13 @@ pkc_status pkc_kv8_reorder(const pkc_kv8_cache* cache, const int* parent, const 
 
 /* One selection step of beam search over B items of K hypotheses (K <= 32):
    the K best of cum[b, j] + log_softmax(logits[b*K + j])[v] over all j and v
-   (ties: the lowest j*V + v), best first. cum, score [B, K] f32 (sums and
-   scores are formed in f64 and rounded once), finished [B, K] uint8 or NULL: a
-   finished hypothesis offers itself alone, with token eos and its score.
+   (ties: the lowest j*V + v), best first. cum, score [B, K] f32. Exponentials
+   are f32 (good to 2^-22 of their values), their sums and the scores f64, in
+   which they are compared; a score is within 2^-21 of the exact one, beside its
+   rounding to f32, and two hypotheses of different rows that are closer than
+   2^-20 may come out in either order (of one row, the logits say). finished
+   [B, K] uint8 or NULL: a finished hypothesis offers itself alone, with token
+   eos and its score.
    parent, token [B, K] int32; finished_out [B, K] (or NULL): token is eos, or
    the parent had finished. A row with a NaN or +inf, or all -inf, and a cum that
    is not finite offer -inf. score may be cum, finished_out may be finished; logits row

@@ -11,10 +11,12 @@
 // Within a row the order is that of the logits, so each CTA reads its row (or
 // its part of one) once from memory and keeps the K largest as keys (ordered
 // value bits over the inverted index); only between rows do the sums matter.
-// Those are kept in f64, and the scores are compared in f64: two hypotheses a
-// few f32 steps apart come out in the order of their exact scores. A cluster
-// holds one item: its CTAs put their lists into the first one's shared memory,
-// which joins them, so there is one launch and no workspace.
+// Those are kept in f64 (of exponentials in f32, good to 2^-22, so their
+// logarithm is too), and the scores are compared in f64: two hypotheses more
+// than 2^-20 apart come out in the order of their exact scores, which at -1000
+// is a 64th of an f32 step. A cluster holds one item: its CTAs put their lists
+// into the first one's shared memory, which joins them, so there is one launch
+// and no workspace.
 //
 // The K largest: the first pass leaves each thread's largest value; each warp
 // sorts its lanes'. K elements reach a warp's K-th, and the least of four warps'

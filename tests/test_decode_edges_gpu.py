@@ -94,6 +94,30 @@ def test_beam_select_infinite_scores(cuda, V):
     assert ((score.double() - rs)[live].abs() <= 2.0 ** -21 + rs[live].abs() * 2.0 ** -24 * 1.01).all()
 
 
+def test_beam_select_close_scores_near_zero(cuda):
+    """Hypotheses whose scores are near zero: a score is within 2^-21 of the
+    exact one (exponentials within 2^-22 of their values), and two that are
+    further apart than twice that come out in their exact order."""
+    import decode_ref
+    import torch
+    B, K, V = 64, 8, 2000
+    g = torch.Generator().manual_seed(8)
+    row = torch.randn(B, 1, V, generator=g).expand(B, K, V).clone()
+    row[:, :, 0] = 30.0
+    row[:, :, 1] = 20.0 + torch.rand(B, K, generator=g)
+    cum = torch.rand(B, K, generator=g) * 2.0 ** -16
+    row, cum = row.to(cuda), cum.to(cuda)
+    no = torch.zeros(B, K, dtype=torch.uint8, device=cuda)
+    score, parent, token, _ = run_select(row, cum, no, V - 1)
+    rs, rp, rt, _ = decode_ref.beam_select(row, cum, no.bool(), V - 1)
+    bound = 2.0 ** -21 + rs.abs() * 2.0 ** -24 * 1.01
+    assert ((score.double() - rs).abs() <= bound).all()
+    # what was picked has, in 64 bits, the score that its place should have, to within the bound of both
+    lp = torch.log_softmax(row.double(), -1) + cum.double()[..., None]
+    picked = lp.flatten(1).gather(1, parent.long() * V + token.long())
+    assert ((picked - rs).abs() <= 2 * 2.0 ** -21).all()
+
+
 def test_beam_reorder_negative_length_is_reported(cuda):
     """A negative length leaves its item as it is and is reported; the other
     items move. A length of zero is no error."""
@@ -112,6 +136,41 @@ def test_beam_reorder_negative_length_is_reported(cuda):
         assert torch.equal(x[1], before[1])
         for b in (0, 2):
             assert torch.equal(x[b], before[b].flip(0))
+
+
+@pytest.mark.parametrize("n", [1, 9])
+def test_kv8_append_beside_a_bad_sequence(cuda, n):
+    """A sequence that is left out (a bad page, length or offset) changes
+    nothing of the other one's: its codes and scales are those of a call of its
+    own."""
+    import torch
+    new = torch.randn(2 * n, 2, 1, 64, generator=torch.Generator().manual_seed(2)).half().to(cuda)
+    alone = make_cache(cuda, 2, [n, n], 1, 64, 16)
+    append(alone, new[:n].contiguous(), [n, 0], [n, 0], max_new=n)
+    assert int(alone["err"]) == 0
+    for what in ("page", "negative page", "length", "short length", "offset"):
+        c = make_cache(cuda, 2, [n, n], 1, 64, 16)
+        mine = int(c["table"][0, 0])
+        lens, n_new = [n, n], [n, n]
+        if what == "page":
+            c["table"][1] = c["total"]
+        elif what == "negative page":
+            c["table"][1] = -5
+        elif what == "length":
+            lens = [n, 16 * c["table"].shape[1] + 1]
+        elif what == "short length":
+            lens = [n, n - 1]
+        else:
+            n_new = [n, n + 3]
+        append(c, new, n_new, lens, max_new=n)
+        assert int(c["err"]) == 110, what
+        for x in "kv":
+            assert torch.equal(c[x][mine], alone[x][mine]), what
+            assert torch.equal(c[x + "_scale"][mine], alone[x + "_scale"][mine]), what
+            others = [p for p in range(c["total"]) if p != mine]
+            assert (c[x][others] == 0x7f).all(), what
+        live = values(c, "k")[mine, 0, :n]
+        assert torch.isfinite(live).all() and (live != 0).any()
 
 
 def test_cross_attention_bound_beyond_a_grid_is_refused(cuda):
