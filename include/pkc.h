@@ -413,10 +413,15 @@ pkc_status pkc_relpos_attention_noalloc(const void* qkv, const void* ptab, int c
 
    What only the device knows is checked there: an offset, length, page or
    parent outside the sizes that the call was given leaves that item (for a
-   page its tokens, for a parent of pkc_beam_reorder its row) out, and the first such error's code goes to *err, a
-   device int that the caller zeroes and reads when it likes (110: out of the
-   sizes, 111: a value that is not a number); err may be NULL. Rows that
-   belong to no item are left as they were.
+   page its tokens, for a parent of pkc_beam_reorder its row) out, and the first
+   such error's code goes to *err, a device int that the caller zeroes and reads
+   when it likes (110: out of the sizes, 111: a value that is not a number); err
+   may be NULL. Rows that belong to no item are left as they were.
+
+   Workspace bytes follow from how a call of these sizes is cut. They do not
+   grow with every size: a call over fewer items may need some where one over
+   more needs none. Ask for each call's own sizes, or take the largest answer
+   over those that will be called with; too small a workspace is refused.
 
    Types: dtype 0 f16, 1 bf16 (beam_select also 2 f32); head_dim 64 or 128;
    n_heads a multiple of n_kv_heads (query head h reads key head
@@ -425,8 +430,10 @@ pkc_status pkc_relpos_attention_noalloc(const void* qkv, const void* ptab, int c
 
 /* Cross attention: item b's query rows [q_off[b], q_off[b+1]) of q attend to
    the kv_len[b] rows of k and v from kv_off[b] on:
-   out = softmax(scale q k^T) v, f32 sums and softmax; an item without keys
-   gives zeros. q, out [q_rows][n_heads][head_dim]; k, v
+   out = softmax(scale q k^T) v; an item without keys gives zeros. Products are
+   summed in f32 and the softmax is taken in f32; each probability is rounded to
+   the type of v (f16 over the 8-bit cache) for its product with v, half a step
+   at most, while the sum that it is divided by is not. q, out [q_rows][n_heads][head_dim]; k, v
    [kv_rows][n_kv_heads][head_dim] (with row strides, so the k | v rows of one
    projection need no copy); q_off [B + 1], kv_off, kv_len [B] int32 on the
    device. max_q and max_kv (up to 2^30) bound the items' rows and keys. All of
@@ -474,7 +481,9 @@ pkc_status pkc_kv8_append(const pkc_kv8_cache* cache, const void* k, long long l
    pkc_cross_attention; max_len (up to 2^30) bounds lens. max_q also chooses
    the kernel: sequences of many new tokens and of one are faster in a call
    each. Value pages of a head may differ in size by any amount; one whose scale
-   is less than 2^-80 of the largest of its sequence may count as zeros. */
+   is less than 2^-80 of the largest of its sequence may count as zeros. bf16
+   queries are brought to f16 by a power of two for each row and head: elements
+   below 2^-14 of the row's largest lose bits (2^-25 of it at most). */
 pkc_status pkc_kv8_attention(const pkc_kv8_cache* cache, const void* q, long long ldq, const int* q_off, int max_q,
                              int q_rows, const int* lens, int max_len, int n_seqs, int n_heads, float scale, int dtype,
                              void* out, long long ldo, void* workspace, size_t workspace_bytes, int* err, void* stream);

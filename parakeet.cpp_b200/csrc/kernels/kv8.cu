@@ -195,8 +195,10 @@ __global__ void __launch_bounds__(128) k_kv8_append_few(const Kv8AppendArgs a, i
 // and neighbouring heads of a row at the same time: a CTA for each head, whose
 // reads are 128 bytes apart from the next ones' by a whole row, reached half
 // the copy rate. 64 sequences of 1 to 1024 tokens, 8 heads of 64, pages of 64:
-// 24 us for 97 MB, 62% of the copy rate (41 us a CTA a head with two reads;
-// 47 us with maxima and checks in f32: the arithmetic on each value counts).
+// 24 us for 97 MB, 62% of the copy rate (41 us a CTA a head with two reads; 47
+// us with maxima and checks in f32: the arithmetic on each value counts). The
+// grid is that of the longest sequence, so half of its CTAs have no page here;
+// 36 bytes a thread are spilled.
 template <typename H, int NV, int WPH>
 __global__ void __launch_bounds__(256, 3) k_kv8_append(const Kv8AppendArgs a, int width, int passes) {
   __shared__ uint32_t s_max[2][8];
