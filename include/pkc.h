@@ -481,9 +481,10 @@ pkc_status pkc_kv8_append(const pkc_kv8_cache* cache, const void* k, long long l
    pkc_cross_attention; max_len (up to 2^30) bounds lens. max_q also chooses
    the kernel: sequences of many new tokens and of one are faster in a call
    each. Value pages of a head may differ in size by any amount; one whose scale
-   is less than 2^-80 of the largest of its sequence may count as zeros. bf16
-   queries are brought to f16 by a power of two for each row and head: elements
-   below 2^-14 of the row's largest lose bits (2^-25 of it at most). */
+   is less than 2^-80 of the largest of its sequence loses bits, or counts as
+   zeros. bf16 queries are brought to f16 by a power of two for each row and
+   head: elements below 2^-14 of the row's largest lose bits (2^-25 of it at
+   most). */
 pkc_status pkc_kv8_attention(const pkc_kv8_cache* cache, const void* q, long long ldq, const int* q_off, int max_q,
                              int q_rows, const int* lens, int max_len, int n_seqs, int n_heads, float scale, int dtype,
                              void* out, long long ldo, void* workspace, size_t workspace_bytes, int* err, void* stream);

@@ -73,7 +73,7 @@ enum : int {
 // What the converting warps tell the softmax about a tile.
 struct TileInfo {
   float4 head;    // the largest key scale (of a tile in one page: its own, negative: a page that is none), what O is
-                  // multiplied by before the tile is added, the exponent that O is kept under behind the tile,
+                  // multiplied by before the tile is added (see move_by), the exponent that O is kept under behind the tile,
                   // parts (1, or the tile's pages)
   float4 ks;      // several pages: key scale of each 16 keys over the largest; negative: a page that is none
   float grow[4];  // and, where it has parts, what O is multiplied by before each
@@ -122,6 +122,10 @@ constexpr int kNoPage = -1000;
 __device__ __forceinline__ float pow2i(int e) {  // 2^e for e <= 127; 0 below 2^-126
   return e < -126 ? 0.f : __int_as_float((e + 127) << 23);
 }
+// What O is multiplied by when its reference moves: 2^e, or -2^(e + 126) for
+// 2^e below 2^-126 (a page 2^80 above the largest so far, which may be 2^80
+// above the reference, still leaves that one's values their bits).
+__device__ __forceinline__ float move_by(int e) { return e < -126 ? -pow2i(e + 126) : pow2i(e); }
 
 template <typename H, bool Q8, int D>
 __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 2)
@@ -359,14 +363,14 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
       tc_fence_after();
       return true;
     };
-    auto scale_o = [&](float f) {
+    auto scale_o = [&](float f, float g) {
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         tmem_ld32(trow + TM_O + 32u * c, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f * g);
         tmem_st32(trow + TM_O + 32u * c, o);
       }
       tmem_st_wait();
@@ -453,12 +457,13 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
       const int parts = Q8 ? (int)ti.w : 1;
 #pragma unroll 1
       for (int j = 0; j < parts && ok; ++j) {
-        const float f = j == 0 ? alpha * ti.y : info(t)->grow[j];
+        const float move = Q8 ? (j == 0 ? ti.y : info(t)->grow[j]) : 1.f;
+        const float f = j == 0 ? alpha * fabsf(move) : fabsf(move);
         const bool scale = pv_buf >= 0 && __any_sync(0xffffffffu, f != 1.f);
         // (a part that is not the tile's first also waits because its arrival
         // below must not count for the part before)
         if ((scale || j > 0) && !(ok = o_settled())) break;
-        if (scale) scale_o(f);
+        if (scale) scale_o(f, Q8 && move < 0.f ? 0x1p-126f : 1.f);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -642,7 +647,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
               if (most != kNoPage && ev - ref <= 7 && ev - ref >= -15) {
                 dv = ev - ref;
               } else {
-                grow = most != kNoPage ? pow2i(ref - ev) : 1.f;
+                grow = most != kNoPage ? move_by(ref - ev) : 1.f;
                 ref = ev;
               }
               most = max(most, ev);
@@ -666,7 +671,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
             } else if (most != kNoPage && mx - ref <= 7 && mn - ref >= -15) {
               if (counts) dv = ev - ref;
             } else if (mx - mn <= 15) {
-              grow = most != kNoPage ? pow2i(ref - mx) : 1.f;
+              grow = most != kNoPage ? move_by(ref - mx) : 1.f;
               ref = mx;
               if (counts) dv = ev - ref;
             } else {
@@ -677,7 +682,7 @@ __global__ void __launch_bounds__(32 * (1 + SOFT_WARPS + (Q8 ? CVT_WARPS : 1)), 
               const uint32_t before = have & ((1u << lane) - 1u);
               const int last = 31 - __clz(have);
               const int prev = __shfl_sync(0xffffffffu, ev, before ? 31 - __clz(before) : 0);
-              grow = !counts ? 1.f : before ? pow2i(prev - ev) : most != kNoPage ? pow2i(ref - ev) : 1.f;
+              grow = !counts ? 1.f : before ? move_by(prev - ev) : most != kNoPage ? move_by(ref - ev) : 1.f;
               ref = __shfl_sync(0xffffffffu, ev, last);
             }
             most = max(most, mx);

@@ -151,3 +151,24 @@ def test_kv8_attention_pages_beyond_all_range(cuda, n, page, exps):
         run_kv8(c, q.view(n, D), [n], [t], 1, out)
         far = torch.tensor([e < max(exps) - 80 for e in exps], device=cuda).repeat_interleave(page)
         check(c, 0, q, out.view(n, 1, D), t, 1, far)
+
+
+@pytest.mark.parametrize("n", [1, 100, 140])
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("exps", [[20, -58, 70], [20, -58, 70, -8, 90], [0, -80, 80], [-40, -120, 30, 30, -45, 100], [10, -65, 60, 60, -15]])
+def test_kv8_attention_falls_then_rises(cuda, n, page, exps):
+    """A page far below the first, then one far above both: a row that sees the
+    first keeps its values, which are no more than 2^80 below the largest."""
+    import torch
+    g = torch.Generator().manual_seed(page + len(exps))
+    for rep in (1, max(1, 64 // page), 2 * max(1, 64 // page)):
+        each = [e for e in exps for _ in range(rep)]
+        if len(each) * page < n:
+            continue
+        for D in (64, 128):
+            c, t = scaled_cache(cuda, page, D, each, g)
+            q = (torch.randn(n, 1, D, generator=g) * 0.5).bfloat16().to(cuda)
+            out = torch.full((n, D), -7.0, dtype=torch.bfloat16, device=cuda)
+            run_kv8(c, q.view(n, D), [n], [t], 1, out)
+            far = torch.tensor([e < max(each) - 80 for e in each], device=cuda).repeat_interleave(page)
+            check(c, 0, q, out.view(n, 1, D), t, 1, far)
