@@ -433,7 +433,9 @@ pkc_status pkc_relpos_attention_noalloc(const void* qkv, const void* ptab, int c
    out = softmax(scale q k^T) v; an item without keys gives zeros. Products are
    summed in f32 and the softmax is taken in f32; each probability is rounded to
    the type of v (f16 over the 8-bit cache) for its product with v, half a step
-   at most, while the sum that it is divided by is not. q, out [q_rows][n_heads][head_dim]; k, v
+   at most, while the sum that it is divided by is not. Products with v are
+   summed before the division, under weights of up to 2^8: values near 2^120 /
+   kv_len and above may overflow f32. q, out [q_rows][n_heads][head_dim]; k, v
    [kv_rows][n_kv_heads][head_dim] (with row strides, so the k | v rows of one
    projection need no copy); q_off [B + 1], kv_off, kv_len [B] int32 on the
    device. max_q and max_kv (up to 2^30) bound the items' rows and keys. All of

@@ -34,14 +34,14 @@
 // is below 2^47 in units of the largest scale, and below 2^127 in those of ref.
 //
 // Measured: 64 x 130 to 384 rows over 250 to 1500 keys, 8 heads of 128: 104 us,
-// 570 TFLOP/s, at 1965 MHz; 122 us on end, where the power cap holds 1645 MHz.
+// 570 TFLOP/s, at 1965 MHz; 120 us on end, where the power cap holds 1645 MHz.
 // A tile takes a CTA 1450 cycles beside the other CTA's; the products alone are
 // 640 for each of the two (a step of 64 columns reads 6 KB of shared memory, 48
 // cycles, for 32 of products), and about 10,000 cycles a CTA lie before its
 // first and behind its last tile. 8 x 100 to 256 new tokens
-// over 300 to 16384 cached ones, 16 heads of 64 for 4, pages of 64: 171 us, 305
+// over 300 to 16384 cached ones, 16 heads of 64 for 4, pages of 64: 174 us, 300
 // TFLOP/s: a tile takes a CTA 2400 cycles and more, of which its softmax warps
-// work 1860 (96 registers, of which 56 to 72 bytes are spilled, beside converting
+// work 1860 (96 registers, of which 56 to 64 bytes are spilled, beside converting
 // warps that use a third of the issue slots) and wait the rest; 53% of the issue
 // slots are used. Two row tiles a CTA under one conversion took 186 us (16-bit
 // keys: 135 instead of 104), three converting warps and 128 registers 169 us but
